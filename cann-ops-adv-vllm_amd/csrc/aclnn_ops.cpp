@@ -10,17 +10,23 @@
 #include <cstdio>
 #include <cstdlib>
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
+#include "../../include/aclnn_append_kv_cache.h"
 #include "../../include/aclnn_assign_block_ids.h"
 #include "../../include/aclnn_cent_select.h"
 #include "../../include/aclnn_compute_cent.h"
+#include "../../include/aclnn_gather_kv_cache.h"
+#include "../../include/aclnn_paged_attention_int4.h"
 #include "../../include/aclnn_select_position.h"
 #include "../../include/aclnn_sparse_paged_attention.h"
 #include "../../include/aclnn_sparse_paged_fusion_attention.h"
+#include "kv_params.h"
 #include "spfa_params.h"
 
 struct aclTensor {
@@ -32,7 +38,7 @@ struct aclTensor {
 struct aclTensorList { std::vector<aclTensor*> items; };
 struct aclIntArray { std::vector<int64_t> v; };
 
-enum OpKind { kOpComputeCent, kOpSelectPosition, kOpCentSelect, kOpAttention, kOpFusion, kOpAssign };
+enum OpKind { kOpComputeCent, kOpSelectPosition, kOpCentSelect, kOpAttention, kOpFusion, kOpAssign, kOpAppend, kOpGather, kOpInt4Attention };
 
 struct aclOpExecutor {
     OpKind op;
@@ -41,6 +47,9 @@ struct aclOpExecutor {
     spfa::SelectParams sel{};
     spfa::AttnParams attn{};
     spfa::AssignParams assign{};
+    spfa::AppendParams append{};
+    spfa::GatherParams gather{};
+    spfa::Int4AttnParams int4{};
     std::vector<long long> act_seq;   // host copy of actualSeqLengths, expanded to B values
     // workspace layout of the two attention ops: [work counters | split arrival counters] (zeroed per launch),
     // split states, per-batch actualSeqLengths
@@ -1482,20 +1491,31 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
     REQUIRE(key && key->items.size() == 1, "key must be a one-tensor list holding the paged K cache");
     const aclTensor* kc = key->items[0];
     REQUIRE(is_contiguous(kc) && kc->data, "key cache must be contiguous device memory");
-    const bool quant = kc->dtype == ACL_INT8;
-    REQUIRE(quant || kc->dtype == l1Cent->dtype, "key cache dtype must equal l1_cent's dtype or be int8");
-    const int es = quant ? 1 : 2;
+    const bool quant = kc->dtype == ACL_INT8, int4 = kc->dtype == ACL_UINT8;
+    REQUIRE(quant || int4 || kc->dtype == l1Cent->dtype, "key cache dtype must equal l1_cent's dtype or be int8 or uint8 (4 bits)");
+    const int es = quant || int4 ? 1 : 2;
     REQUIRE(blockSize > 0 && blockSize <= 512, "blockSize %lld out of (0, 512]", (long long)blockSize);
     const int bs = (int)blockSize;
     const auto& kd = kc->dims;
     bool bsh;
-    if (kd.size() == 3 && kd[1] == bs && kd[2] == (int64_t)Hkv * D) bsh = true;
+    if (int4) {
+        // codes [blocks, Hkv, bs, D / 2]; antiquantScale holds the tokens' (scale, zero) pairs
+        REQUIRE(D <= 256 && bs % 16 == 0, "4-bit key cache: head dim %d (32 .. 256), blockSize %d (a multiple of 16)", D, bs);
+        REQUIRE(kd.size() == 4 && kd[1] == Hkv && kd[2] == bs && kd[3] == D / 2, "4-bit key cache must be [blocks, Hkv, bs, D / 2]");
+        REQUIRE(!absent(antiquantScale) && antiquantScale->dtype == ACL_FLOAT16 && antiquantScale->dims.size() == 4 &&
+                    antiquantScale->dims[0] == kd[0] && antiquantScale->dims[1] == Hkv && antiquantScale->dims[2] == bs &&
+                    antiquantScale->dims[3] == 2 && is_contiguous(antiquantScale),
+                "a 4-bit key cache needs antiquantScale: its parameters, contiguous float16 [blocks, Hkv, bs, 2]");
+        REQUIRE(absent(antiquantOffset), "antiquantOffset must be absent with a 4-bit key cache (its zeros are in antiquantScale)");
+        bsh = false;
+    }
+    else if (kd.size() == 3 && kd[1] == bs && kd[2] == (int64_t)Hkv * D) bsh = true;
     else if (kd.size() == 4 && kd[1] == bs && kd[2] == Hkv && kd[3] == D) bsh = true;
     else if (kd.size() == 4 && kd[1] == Hkv && kd[2] == bs && kd[3] == D) bsh = false;
     else return fail(ACLNN_ERR_PARAM_INVALID, "key cache must be [blocks,bs,Hkv*D], [blocks,bs,Hkv,D] or [blocks,Hkv,bs,D]");
     REQUIRE(kd[0] > 0 && kd[0] <= 0x7fffffff, "key cache has no blocks");
     const int lpt = D * es / 16;
-    REQUIRE(lpt >= 4 && lpt <= 64, "head dim %d with %d-byte elements is not supported (row bytes 64 .. 1024)", D, es);
+    REQUIRE(int4 || lpt >= 4 && lpt <= 64, "head dim %d with %d-byte elements is not supported (row bytes 64 .. 1024)", D, es);
     aclOpExecutor* e = new aclOpExecutor();
     e->op = kOpAssign;
     spfa::AssignParams& p = e->assign;
@@ -1512,16 +1532,20 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
         p.antiq_per_tensor = per_tensor ? 1 : 0;
         p.antiq_scale = data_ptr(antiquantScale);
         p.antiq_offset = absent(antiquantOffset) ? nullptr : data_ptr(antiquantOffset);
+    } else if (int4) {
+        p.key_params = data_ptr(antiquantScale);
     } else if (!absent(antiquantScale) || !absent(antiquantOffset)) {
         return bail(fail(ACLNN_ERR_PARAM_INVALID, "antiquant parameters given but the key cache is not int8"));
     }
     p.kcache = data_ptr(kc);
-    if (bsh) {
+    if (int4) {
+        p.tok_stride = D / 2; p.head_stride = (long long)bs * D / 2; p.blk_stride = (long long)Hkv * bs * D / 2;
+    } else if (bsh) {
         p.blk_stride = (long long)bs * Hkv * D * es; p.tok_stride = (long long)Hkv * D * es; p.head_stride = (long long)D * es;
     } else {
         p.blk_stride = (long long)Hkv * bs * D * es; p.head_stride = (long long)bs * D * es; p.tok_stride = (long long)D * es;
     }
-    p.kv_dtype = to_dtype(kc->dtype);
+    p.kv_dtype = int4 ? (int)spfa::kI4 : to_dtype(kc->dtype);
     p.n_blocks = (int)kd[0];
     p.cent = data_ptr(l1Cent);
     p.qk_dtype = to_dtype(l1Cent->dtype);
@@ -1597,5 +1621,7 @@ aclnnStatus aclnnSparsePagedFusionAttentionNoAlloc(aclOpExecutor* executor, cons
     if (!capturing) __atomic_store_n(&g_noalloc_zeroed[dev], err == hipSuccess, __ATOMIC_RELEASE);
     return finish(executor, err, "sparse_paged_fusion_attention launch (built-in scratch)");
 }
+
+#include "aclnn_kv_ops.inc"
 
 }  // extern "C"

@@ -1,0 +1,867 @@
+// Attention over a paged cache held in 4 bits (gfx950).
+//
+//   K_t = s_t c_t + z_t,  V_t = s'_t c'_t + z'_t    (codes c, c' in 0 .. 15; s, z per token and kv head, float16)
+//   score(n, t) = scale (s_t (q_n . c_t) + z_t sum(q_n)),   O_n = (sum_t (p_t s'_t) c'_t + sum_t p_t z'_t) / sum_t p_t
+//
+// so the matrix cores multiply CODES and the parameters are applied to scores and probabilities, one fma each.  A code
+// becomes a matrix operand by masking alone: (w & 0x000f000f) are two codes in the bits of float16 denormals c * 2^-24
+// (the matrix cores take denormals as they are; the odd codes of a byte come out 16 times larger, which the q elements
+// they meet and the final scaling take back).  Five vector instructions unpack eight codes.
+//
+// Per step of 32 tokens a wave computes, with v_mfma_f32_16x16x32_f16 (A = K codes of 16 tokens, B = 16 q rows):
+//   S^T[token, row]: lane l holds row l % 16 and the tokens 4 (l / 16) .. + 3 of each half of the step;
+//   O^T[channel, row] += V^T[channel, token] P^T[token, row]: the probabilities are already where operand B wants them
+//   (tokens 4 (l / 16) .. + 3 of both halves = its eight k slots), nothing crosses lanes between the two products.
+//
+// The running maximum is lazy: a row keeps a reference m that is at most 8 (log2) below its true maximum, and a step
+// that would exceed that (or whose V scales outgrow the reference scale R that keeps p * s' inside float16) takes the
+// slow path, which moves m and R and rescales the sums.  Sums, statistics and O are float32; p * s' is rounded to
+// float16 (relative 2^-11, down to 2^-20 of the peak) for the second product.
+//
+// Work.  An item is (sequence, kv head, tile of q rows); its tokens are cut into steps of 32 tokens.  All items' steps
+// form one line that is cut into equal pieces, one per resident workgroup: lengths may be as ragged as they like.  A
+// workgroup computes its piece from seq_len alone.  An item that spans several workgroups is merged by the last of them
+// to arrive (partial states in the workspace, one arrival counter per split item).
+//   by tokens (few rows): the four waves of a workgroup take every fourth step, states merged through LDS;
+//   by rows (prompts): the four waves hold different rows and walk the same tokens (shared through the L1 cache).
+// With page lists (one row of q per sequence) an item is (sequence, list) and workers workgroups share each list.
+#include "kv_params.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+namespace spfa {
+namespace {
+
+#include "spfa_common.inc"
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -3.0e38f;          // reference of a row that has seen no token
+constexpr float kLazy = 8.f;                // log2 distance a reference may fall behind the true maximum
+constexpr int kScaleTop = 6;                // V scales are brought below 2^6 (and may grow to 2^7 before the next slow path)
+
+// A step: for each half of 16 tokens the physical page (< 0: nothing there), the row in it and the token's place in the
+// sequence.
+struct Ptrs { int phys[2], row[2], tok[2]; };
+
+template <int W> struct Words { uint32_t w[W]; };
+template <int W>
+__device__ __forceinline__ Words<W> load_words(const uint8_t* p) {
+    Words<W> r;
+    if constexpr (W == 1) r.w[0] = *(const uint32_t*)p;
+    else if constexpr (W == 2) { const uint2 v = *(const uint2*)p; r.w[0] = v.x; r.w[1] = v.y; }
+    else {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const uint4 v = *(const uint4*)(p + 16 * i);
+            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+        }
+    }
+    return r;
+}
+
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+// eight codes of a word as four operand words: nibbles (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ u32x4 codes_of(uint32_t w) {
+    const uint32_t h = w >> 8;
+    return u32x4{w & 0x000f000fu, w & 0x00f000f0u, h & 0x000f000fu, h & 0x00f000f0u};
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {   // round to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, half2v));
+}
+__device__ __forceinline__ float lo16(uint32_t w) { return f16_bits((uint16_t)(w & 0xffffu)); }
+__device__ __forceinline__ float hi16(uint32_t w) { return f16_bits((uint16_t)(w >> 16)); }
+
+// Sums / maxima over the four lane groups that hold the same row.
+__device__ __forceinline__ float rows_sum(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
+__device__ __forceinline__ float rows_max(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
+
+// ---- the line of steps ----------------------------------------------------------------------------------------------
+// rows of a sequence: first row of the call, how many; its tokens, and those that its table can hold
+struct Seq { int first, n, tokens, len; };
+__device__ __forceinline__ Seq seq_of(const TokenMap& m, int b) {
+    Seq s;
+    s.first = m.query_start ? m.query_start[b] : b;
+    const int end = m.query_start ? min(m.query_start[b + 1], m.T) : b + 1;
+    s.first = max(s.first, 0);
+    s.n = max(end - s.first, 0);
+    s.tokens = max(m.seq_len[b], 0);
+    s.len = (int)min((long long)s.tokens, (long long)m.max_page * m.block_size);
+    return s;
+}
+// Tokens that row i of a sequence sees: its position is seq_len - n + i, and nothing lies behind the table.
+__device__ __forceinline__ int seen_by(const Int4AttnParams& p, const Seq& s, int i) {
+    return p.causal ? max(0, min(s.len, s.tokens - s.n + i + 1)) : s.len;
+}
+__device__ __forceinline__ int steps_of(const Int4AttnParams& p, const Seq& s, int rt) {
+    const int last = min((rt + 1) * p.rows_tile, s.n * p.G) - 1;
+    return max(1, (seen_by(p, s, last / p.G) + kInt4StepTokens - 1) / kInt4StepTokens);
+}
+__device__ __forceinline__ int row_tiles(const Int4AttnParams& p, const Seq& s) { return (s.n * p.G + p.rows_tile - 1) / p.rows_tile; }
+
+__device__ __forceinline__ long long wave_sum(long long x) {
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ __forceinline__ long long wave_scan(long long x, int lane) {   // inclusive
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long up = __shfl_up(x, d);
+        if (lane >= d) x += up;
+    }
+    return x;
+}
+// steps of one kv head of a sequence (all its row tiles), computed by one lane / by the wave
+__device__ __forceinline__ long long head_steps_lane(const Int4AttnParams& p, const Seq& s) {
+    const int nt = row_tiles(p, s);
+    if (nt <= 0) return 0;
+    if (!p.causal) return (long long)nt * steps_of(p, s, 0);
+    long long t = 0;
+    for (int rt = 0; rt < nt; ++rt) t += steps_of(p, s, rt);
+    return t;
+}
+__device__ __forceinline__ long long head_steps_wave(const Int4AttnParams& p, const Seq& s, int lane) {
+    const int nt = row_tiles(p, s);
+    if (!p.causal) return nt > 0 ? (long long)nt * steps_of(p, s, 0) : 0;
+    long long t = 0;
+    for (int rt = lane; rt < nt; rt += 64) t += steps_of(p, s, rt);
+    return wave_sum(t);
+}
+
+// ---- the state of a wave -------------------------------------------------------------------------------------------
+template <int D, int NT>
+struct State {
+    f32x4 o[NT][D / 16];     // [2 j + parity][i]: channel (4 kg + i) * D / 16 + 2 j + parity, in units of the codes
+    float m[NT], l[NT], z[NT];
+    float inv_r;             // power of two: V scales are taken times inv_r
+    int seen;                // bit t: the lane's row of tile t has seen a token
+    int open;                // wave-uniform, bit 0: some row has seen none, bit 1: no V scale above 0 so far
+};
+template <int D, int NT>
+__device__ __forceinline__ void clear_state(State<D, NT>& S) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        S.m[t] = S.l[t] = S.z[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) S.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    S.inv_r = 1.f;
+    S.seen = 0;
+    S.open = 3;
+}
+
+template <int D, int NT>
+struct Query {
+    u32x4 q[NT][D / 32];     // operand B: k slots in the order of codes_of
+    float sum[NT];           // sum(q) * scale * log2(e)
+    int lim[NT];             // tokens the lane's row sees
+    float ks;                // what a score in code units is multiplied by (besides s_t)
+    int lim_min, lim_max;    // fewest / most tokens a live row of the wave sees
+};
+
+// What the rows of a work item are: row r is token first + r / G of the sequence, q head head0 + r % G.
+struct Rows { int first, head0, G, kvh, n; };
+
+// q rows [row0, row0 + 16 NT) of an item -> operand B.  The rows of a wave are brought to a common power of two with the
+// largest element in [2^10, 2^11): float16 then holds every element down to 2^-25 of it exactly (bfloat16 rows outside
+// float16's range included), and the even slots, 16 times larger, stay below 2^15.
+template <int D, int NT>
+__device__ __forceinline__ void load_query(const Int4AttnParams& p, const Seq& s, const Rows& R, int row0, Query<D, NT>& Q, int lane) {
+    constexpr int W = D / 32, E = 8 * W;      // words / channels of a lane
+    const int n = lane & 15, kg = lane >> 4;
+    const bool bf = p.q_dtype == kBF16;
+    uint32_t raw[NT][E / 2];
+    float top = 0.f;
+    Q.lim_min = 0x7fffffff;
+    Q.lim_max = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n;
+        const bool live = r < R.n;
+        const int i = live ? r / R.G : 0, g = live ? r - i * R.G : 0;
+        const uint16_t* src = (const uint16_t*)p.q + (long long)(R.first + i) * p.q_tok + (long long)(R.head0 + g) * p.q_head + kg * E;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) raw[t][e] = 0u;
+        if (live && p.q_wide) {
+#pragma unroll
+            for (int e = 0; e < E / 8; ++e) {
+                const uint4 v = *(const uint4*)(src + 8 * e);
+                raw[t][4 * e] = v.x; raw[t][4 * e + 1] = v.y; raw[t][4 * e + 2] = v.z; raw[t][4 * e + 3] = v.w;
+            }
+        } else if (live) {
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) raw[t][e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+        }
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+            const float a = bf ? bf16_lo(raw[t][e]) : lo16(raw[t][e]), b = bf ? bf16_hi(raw[t][e]) : hi16(raw[t][e]);
+            sum += a + b;
+            top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+        }
+        Q.sum[t] = rows_sum(sum) * (p.scale * kLog2e);
+        Q.lim[t] = live ? seen_by(p, s, i) : 0;
+        if (live) {
+            Q.lim_min = min(Q.lim_min, Q.lim[t]);
+            Q.lim_max = max(Q.lim_max, Q.lim[t]);
+        }
+    }
+    for (int d = 1; d < 64; d <<= 1) {
+        top = fmaxf(top, __shfl_xor(top, d));
+        Q.lim_min = min(Q.lim_min, __shfl_xor(Q.lim_min, d));
+        Q.lim_max = max(Q.lim_max, __shfl_xor(Q.lim_max, d));
+    }
+    Q.lim_min = __builtin_amdgcn_readfirstlane(Q.lim_min);
+    Q.lim_max = __builtin_amdgcn_readfirstlane(Q.lim_max);
+    // exponent of the largest element (an infinite query is not scaled: its row comes out NaN)
+    const int eb = (int)((__float_as_uint(top) >> 23) & 255u);
+    int up = (top > 0.f && eb < 255) ? 127 + 10 - eb : 0;
+    up = __builtin_amdgcn_readfirstlane(max(-118, min(118, up)));
+    const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+    // codes arrive as c * 2^-24 (even channels) and 16 c * 2^-24 (odd); even slots of q carry 16 f, odd ones f
+    Q.ks = p.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;   // 2^24 / 16
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = raw[t][4 * j + e];
+                x[2 * e] = (bf ? bf16_lo(w) : lo16(w)) * (16.f * f);
+                x[2 * e + 1] = (bf ? bf16_hi(w) : hi16(w)) * f;
+            }
+            Q.q[t][j] = u32x4{pack_f16(x[0], x[4]), pack_f16(x[1], x[5]), pack_f16(x[2], x[6]), pack_f16(x[3], x[7])};
+        }
+}
+
+// The data of one step.
+template <int D>
+struct Tile {
+    Words<D / 32> k[2], v[2];
+    u32x4 kp[2], vp[2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_tile(const Int4AttnParams& p, int kvh, const Ptrs& a, Tile<D>& t, int lane) {
+    constexpr int W = D / 32;
+    const int n = lane & 15, kg = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const long long row = ((long long)max(a.phys[i], 0) * p.Hkv + kvh) * p.map.block_size + a.row[i];
+        const uint8_t* kb = p.kcache + row * (D / 2);
+        const uint8_t* vb = p.vcache + row * (D / 2);
+        t.k[i] = load_words<W>(kb + (unsigned)(n * (D / 2) + kg * 4 * W));
+        t.v[i] = load_words<W>(vb + (unsigned)(kg * (D / 2 * 4) + n * 4 * W));
+        t.kp[i] = *(const u32x4*)((const uint8_t*)(p.k_params + row) + (unsigned)(kg * 16));
+        t.vp[i] = *(const u32x4*)((const uint8_t*)(p.v_params + row) + (unsigned)(kg * 16));
+    }
+}
+
+// One step of a wave.  MASKED: some token of the step is hidden from some row (the end of the sequence, the causal
+// border, a page that is not there); a hidden token counts as probability 0 whatever its parameters hold.
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ void attend(const Query<D, NT>& Q, State<D, NT>& S, const Tile<D>& T, const Ptrs& a, int seq_end, int lane) {
+    constexpr int W = D / 32;
+    const int kg = lane >> 4;
+    f32x4 s[2][NT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const u32x4 c = codes_of(T.k[i].w[j]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[i][t] = mfma(c, Q.q[t][j], s[i][t]);
+        }
+    }
+    float vs[2][4], vs_top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int tok = a.tok[i] + 4 * kg + e;
+            const bool there = !MASKED || (a.phys[i] >= 0 && tok < seq_end);
+            vs[i][e] = there ? lo16(T.vp[i][e]) * S.inv_r : 0.f;
+            vs_top = fmaxf(vs_top, vs[i][e]);
+        }
+    // scores relative to the rows' references (log2)
+    float x_top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ks = lo16(T.kp[i][e]) * Q.ks, kz = hi16(T.kp[i][e]);
+            const int tok = a.tok[i] + 4 * kg + e;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x = fmaf(s[i][t][e], ks, fmaf(kz, Q.sum[t], -S.m[t]));
+                if (MASKED && (a.phys[i] < 0 || tok >= min(seq_end, Q.lim[t]))) x = -__builtin_inff();
+                s[i][t][e] = x;
+                x_top = fmaxf(x_top, x);
+            }
+        }
+    if (MASKED || S.open || __any(x_top > kLazy || vs_top > (float)(2 << kScaleTop))) {
+        // move the references: rows to their true maxima, the scale reference where it is free or outgrown
+        float vmax = fminf(vs_top, 3.0e38f);
+        for (int d = 1; d < 64; d <<= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, d));
+        float r = 1.f;
+        if (vmax > (float)(2 << kScaleTop) || ((S.open & 2) && vmax > 0.f)) {
+            const int e = max(-60, min(60, (int)((__float_as_uint(vmax) >> 23) & 255u) - 127 + 1 - kScaleTop));
+            r = __uint_as_float((uint32_t)(127 - e) << 23);   // vmax * r in [2^5, 2^6)
+            S.open &= 1;
+        }
+        S.inv_r *= r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vs[i][e] *= r;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][t][e]);
+            top = rows_max(top);
+            const bool before = (S.seen >> t) & 1, now = top > -__builtin_inff();
+            const float up = before ? fmaxf(top, 0.f) : (now ? top : 0.f);
+            const float alpha = before ? fast_exp2(-up) : 1.f;      // (nothing is in the sums before the first token)
+            S.m[t] += up;
+            S.l[t] *= alpha;
+            S.z[t] *= alpha;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) S.o[t][d] *= alpha * r;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][t][e] -= up;
+            if (now) S.seen |= 1 << t;
+        }
+        const int none = __any(S.seen != (1 << NT) - 1) ? 1 : 0;
+        S.open = __builtin_amdgcn_readfirstlane((S.open & 2) | none);
+    }
+    // probabilities; P^T operand: tokens (0, 2), (1, 3) of the lane's four, first half then second half
+    u32x4 pb[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float w[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = s[i][t][e], pr = fast_exp2(x), vz = hi16(T.vp[i][e]);
+                const bool hidden = MASKED && x == -__builtin_inff();
+                S.l[t] += pr;
+                S.z[t] = hidden ? S.z[t] : fmaf(pr, vz, S.z[t]);
+                w[i][e] = hidden ? 0.f : pr * vs[i][e];
+            }
+        pb[t] = u32x4{pack_f16(w[0][0], w[0][2]), pack_f16(w[0][1], w[0][3]), pack_f16(w[1][0], w[1][2]), pack_f16(w[1][1], w[1][3])};
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const u32x4 c0 = codes_of(T.v[0].w[j]), c1 = codes_of(T.v[1].w[j]);
+        const u32x4 even = {c0[0], c0[2], c1[0], c1[2]}, odd = {c0[1], c0[3], c1[1], c1[3]};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            S.o[t][2 * j] = mfma(even, pb[t], S.o[t][2 * j]);
+            S.o[t][2 * j + 1] = mfma(odd, pb[t], S.o[t][2 * j + 1]);
+        }
+    }
+}
+
+// ---- finished states ------------------------------------------------------------------------------------------------
+// Per row: D un-normalised outputs, the reference m (log2) and the sum l; a row without tokens has m = kNoMax, l = 0.
+// In registers of a wave: State with o in real units and m, l complete in every lane of the row.
+template <int D, int NT>
+__device__ __forceinline__ void settle(State<D, NT>& S) {
+    const float even = 16777216.f / S.inv_r, odd = even * 0.0625f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        S.l[t] = rows_sum(S.l[t]);
+        const float z = rows_sum(S.z[t]);
+        if (!((S.seen >> t) & 1) && !(S.l[t] != S.l[t])) S.m[t] = kNoMax;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S.o[t][d][i] = S.o[t][d][i] * ((d & 1) ? odd : even) + z;
+    }
+}
+// channel of o[.][d][i] in a lane: kg * D / 4 + i * D / 16 + d
+template <int D, int NT>
+__device__ __forceinline__ void state_to_lds(const State<D, NT>& S, float* st, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float* row = st + (16 * t + n) * (D + 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) row[kg * (D / 4) + i * (D / 16) + d] = S.o[t][d][i];
+        if (kg == 0) { row[D] = S.m[t]; row[D + 1] = S.l[t]; }
+    }
+}
+template <int D, int NT>
+__device__ __forceinline__ void merge_from_lds(State<D, NT>& S, const float* st, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float* row = st + (16 * t + n) * (D + 2);
+        const float mo = row[D], lo = row[D + 1], m = fmaxf(S.m[t], mo);
+        const float a = fast_exp2(S.m[t] - m), b = fast_exp2(mo - m);
+        S.m[t] = m;
+        S.l[t] = S.l[t] * a + lo * b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) S.o[t][d][i] = S.o[t][d][i] * a + row[kg * (D / 4) + i * (D / 16) + d] * b;
+    }
+}
+
+__device__ __forceinline__ void put_out(const Int4AttnParams& p, long long at, float a, float b) {
+    if (p.out_dtype == kF32) *(float2*)((float*)p.out + at) = make_float2(a, b);
+    else if (p.out_dtype == kBF16)
+        *(uint32_t*)((uint16_t*)p.out + at) = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
+    else *(uint32_t*)((uint16_t*)p.out + at) = pack_f16(a, b);
+}
+__device__ __forceinline__ float out_factor(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -3.4e38f : (m + __log2f(l)) * 0.6931471805599453f; }
+
+template <int D, int NT>
+__device__ __forceinline__ void write_out(const Int4AttnParams& p, const Rows& R, int row0, const State<D, NT>& S, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n;
+        if (r >= R.n) continue;
+        const int i0 = r / R.G, head = R.head0 + r - i0 * R.G;
+        const long long row = (long long)(R.first + i0) * p.Hq + head;
+        const float f = out_factor(S.l[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 16; d += 2)
+                put_out(p, row * D + kg * (D / 4) + i * (D / 16) + d, S.o[t][d][i] * f, S.o[t][d + 1][i] * f);
+        if (p.lse && kg == 0) p.lse[row] = lse_of(S.m[t], S.l[t]);
+    }
+}
+
+union Pair { unsigned long long u; float f[2]; };
+__device__ __forceinline__ void st_pair(float* ptr, float a, float b) {
+    Pair v;
+    v.f[0] = a; v.f[1] = b;
+    st_agent((unsigned long long*)ptr, v.u);
+}
+__device__ __forceinline__ Pair ld_pair(const float* ptr) {
+    Pair v;
+    v.u = ld_agent((const unsigned long long*)ptr);
+    return v;
+}
+template <int D, int NT>
+__device__ __forceinline__ void state_to_parts(const State<D, NT>& S, float* st, int row0, int n_rows, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n;
+        if (r >= n_rows) continue;
+        float* row = st + (long long)r * (D + 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 16; d += 2) st_pair(row + kg * (D / 4) + i * (D / 16) + d, S.o[t][d][i], S.o[t][d + 1][i]);
+        if (kg == 0) st_pair(row + D, S.m[t], S.l[t]);
+    }
+}
+
+// The last workgroup to arrive at a split item merges its np partial states, which lie `stride` floats apart except for
+// the first.  D / 4 threads share a row, four channels each; where rows are fewer than the 1024 / D groups of threads,
+// several groups take every sub-th part of a row and join through LDS.
+template <int D>
+__device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows& R, int row0, int n_rows, const float* first,
+                                            const float* rest, long long stride, int np, float* lds) {
+    constexpr int TPR = D / 4, SLOTS = 256 / TPR, BATCH = 8;
+    const int slot = threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
+    int sub = 1;
+    while (sub * 2 * n_rows <= SLOTS && sub * 2 <= np) sub *= 2;
+    const int per_pass = SLOTS / sub, sid = slot % sub;
+    for (int base = 0; base < n_rows; base += per_pass) {
+        const int r = base + slot / sub;
+        const bool live = r < n_rows;
+        float m = kNoMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = sid; p0 < np && live; p0 += BATCH * sub) {
+            Pair ml[BATCH], a[BATCH], b[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int j = min(p0 + u * sub, np - 1);
+                const float* row = (j == 0 ? first : rest + (long long)(j - 1) * stride) + (long long)r * (D + 2);
+                ml[u] = ld_pair(row + D);
+                a[u] = ld_pair(row + c);
+                b[u] = ld_pair(row + c + 2);
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) top = fmaxf(top, ml[u].f[0]);
+            const float keep = fast_exp2(m - top);
+            m = top;
+            l *= keep;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const float f = p0 + u * sub < np ? fast_exp2(ml[u].f[0] - top) : 0.f;
+                if (p0 + u * sub < np) {
+                    l += ml[u].f[1] * f;
+                    o[0] += a[u].f[0] * f; o[1] += a[u].f[1] * f; o[2] += b[u].f[0] * f; o[3] += b[u].f[1] * f;
+                }
+            }
+        }
+        if (sub > 1) {
+            float* st = lds + slot * (D + 2);
+            __syncthreads();
+            if (sid != 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st[c + e] = o[e];
+                if (c == 0) { st[D] = m; st[D + 1] = l; }
+            }
+            __syncthreads();
+            if (sid == 0)
+                for (int u = 1; u < sub; ++u) {
+                    const float* ot = lds + (slot + u) * (D + 2);
+                    const float mo = ot[D], lo = ot[D + 1], top = fmaxf(m, mo), f = fast_exp2(m - top), g = fast_exp2(mo - top);
+                    m = top;
+                    l = l * f + lo * g;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + ot[c + e] * g;
+                }
+        }
+        if (live && sid == 0) {
+            const int rr = row0 + r, i0 = rr / R.G, head = R.head0 + rr - i0 * R.G;
+            const long long row = (long long)(R.first + i0) * p.Hq + head;
+            const float f = out_factor(l);
+            put_out(p, row * D + c, o[0] * f, o[1] * f);
+            put_out(p, row * D + c + 2, o[2] * f, o[3] * f);
+            if (p.lse && c == 0) p.lse[row] = lse_of(m, l);
+        }
+    }
+}
+
+// ---- the kernel -----------------------------------------------------------------------------------------------------
+template <int D, int NT, bool ROWS, bool LIST>
+struct Lds {
+    static constexpr int merge = ROWS ? 0 : 2 * 16 * NT * (D + 2) * 4;
+    static constexpr int join = (1024 / D) * (D + 2) * 4;
+    static constexpr int fixed = (merge > join ? merge : join) + 16;
+};
+
+// Steps [s0, s1) of an item for this wave (every fourth one from s0 + wave, or all of them with ROWS).
+template <int D, int NT, bool ROWS, bool LIST>
+__device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, const Query<D, NT>& Q, State<D, NT>& S,
+                                     int s0, int s1, const int2* list, int n_list, int wave, int lane) {
+    const int stride = ROWS ? 1 : 4;
+    const int seq_end = sq.len;
+    int s = ROWS ? s0 : s0 + wave;
+    // no row of the wave sees anything from lim_max on (lists are not ordered by position: all of theirs is walked)
+    if (!LIST) s1 = min(s1, (min(Q.lim_max, seq_end) + kInt4StepTokens - 1) / kInt4StepTokens);
+    if (s >= s1) return;
+    const int32_t* table = p.map.block_table + (long long)b * p.map.max_page;
+    const int bs = p.map.block_size;
+    // page and row of 16 tokens: (units of 16) * ceil(2^32 / (bs / 16)) >> 32, exact below 2^22 units
+    auto locate = [&](int step, Ptrs& a) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const unsigned u = 2u * (unsigned)step + i;
+            const int page = (int)(p.page_magic ? __umulhi(u, p.page_magic) : u);
+            a.row[i] = (int)(16u * u) - page * bs;
+            if (LIST) {
+                const int2 e = page < n_list ? list[page] : make_int2(0, -1);
+                a.tok[i] = __builtin_amdgcn_readfirstlane(e.x) * bs + a.row[i];
+                a.phys[i] = e.y;
+            } else {
+                a.tok[i] = (int)(16u * u);
+                a.phys[i] = a.tok[i] < seq_end ? table[page] : -1;
+            }
+        }
+    };
+    auto fix = [&](Ptrs& a) {     // the table entries have arrived
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int e = __builtin_amdgcn_readfirstlane(a.phys[i]);
+            a.phys[i] = (e >= 0 && e < p.map.n_blocks) ? e : -1;
+        }
+    };
+    auto step_of = [&](const Tile<D>& T, const Ptrs& a) {
+        const bool masked = a.phys[0] < 0 || a.phys[1] < 0 || a.tok[0] + 16 > min(seq_end, Q.lim_min) || a.tok[1] + 16 > min(seq_end, Q.lim_min);
+        if (masked) attend<D, NT, true>(Q, S, T, a, seq_end, lane);
+        else attend<D, NT, false>(Q, S, T, a, seq_end, lane);
+    };
+    Tile<D> t0, t1;
+    Ptrs a0, a1;
+    locate(s, a0);
+    if (s + stride < s1) locate(s + stride, a1);
+    fix(a0);
+    load_tile<D>(p, R.kvh, a0, t0, lane);
+    while (true) {
+        Ptrs next;
+        const bool one = s + stride < s1, two = s + 2 * stride < s1;
+        if (two) locate(s + 2 * stride, next);
+        if (one) {
+            fix(a1);
+            load_tile<D>(p, R.kvh, a1, t1, lane);
+        }
+        step_of(t0, a0);
+        if (!one) break;
+        t0 = t1;
+        a0 = a1;
+        a1 = next;
+        s += stride;
+    }
+}
+
+// One item, steps [s0, s1) of n_steps: the whole of it is written out, a part goes to the workspace and the last
+// workgroup to arrive merges.  part: where this workgroup's state goes; first / rest / stride / np: where all of them are.
+template <int D, int NT, bool ROWS, bool LIST>
+__device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, int row0, int s0, int s1, bool whole,
+                                         float* part, const float* first, const float* rest, long long stride, int np,
+                                         unsigned* counter, const int2* list, int n_list, float* lds, int* flag, int wave, int lane) {
+    const int my_row0 = row0 + (ROWS ? wave * 16 * NT : 0);
+    const int n_rows = min(p.rows_tile, R.n - row0);
+    State<D, NT> S;
+    clear_state(S);
+    {
+        Query<D, NT> Q;
+        load_query<D, NT>(p, sq, R, my_row0, Q, lane);
+        walk<D, NT, ROWS, LIST>(p, sq, b, R, Q, S, s0, s1, list, n_list, wave, lane);
+    }
+    settle<D, NT>(S);
+    if (!ROWS) {
+        float* other = lds + 16 * NT * (D + 2);
+        __syncthreads();                                  // the areas may still be read for the item before
+        if (wave & 1) state_to_lds<D, NT>(S, wave == 1 ? lds : other, lane);
+        __syncthreads();
+        if (!(wave & 1)) merge_from_lds<D, NT>(S, wave == 0 ? lds : other, lane);
+        __syncthreads();
+        if (wave == 2) state_to_lds<D, NT>(S, lds, lane);
+        __syncthreads();
+        if (wave == 0) merge_from_lds<D, NT>(S, lds, lane);
+    }
+    const bool mine = ROWS || wave == 0;
+    if (whole) {
+        if (mine) write_out<D, NT>(p, R, my_row0, S, lane);
+        return;
+    }
+    if (mine) state_to_parts<D, NT>(S, part, my_row0 - row0, n_rows, lane);
+    wait_stores();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        *flag = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == np - 1;
+    __syncthreads();
+    const int last = *flag;
+    if (last) {
+        if (threadIdx.x == 0) st_agent(counter, 0u);      // left as found: the next launch on this workspace counts again
+        merge_parts<D>(p, R, row0, n_rows, first, rest, stride, np, lds);
+    }
+    __syncthreads();
+}
+
+template <int D, int NT, bool ROWS, bool LIST>
+__global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_attention_kernel(const Int4AttnParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* lds = (float*)smem;
+    int* flag = (int*)(smem + Lds<D, NT, ROWS, LIST>::fixed - 16);
+    const int lane = lane_id(), wave = wave_id();
+    const long long state = (long long)p.rows_tile * (D + 2);
+
+    if constexpr (LIST) {
+        const int item = blockIdx.x / p.workers, share = blockIdx.x - item * p.workers;
+        const int b = item / p.list_rows, lr = item - b * p.list_rows;
+        const Seq sq = seq_of(p.map, b);
+        const bool per_head = p.list_rows == p.Hq;
+        const Rows R{sq.first, per_head ? lr : lr * p.G, per_head ? 1 : p.G, per_head ? lr / p.G : lr, per_head ? 1 : p.G};
+        int2* list = (int2*)(smem + Lds<D, NT, ROWS, LIST>::fixed);
+        // a list ends at its first entry outside the table (the sentinel among them): the shortest over the threads
+        if (threadIdx.x == 0) *flag = p.P;
+        __syncthreads();
+        const int32_t* src = p.lists + ((long long)b * p.list_rows + lr) * p.P;
+        int end = p.P;
+        for (int j = threadIdx.x; j < p.P; j += 256) {
+            const int lp = src[j];
+            const bool ok = lp >= 0 && lp < p.map.max_page;
+            list[j] = make_int2(ok ? lp : 0, ok ? p.map.block_table[(long long)b * p.map.max_page + lp] : -1);
+            if (!ok && j < end) end = j;
+        }
+        if (end < p.P) atomicMin(flag, end);
+        __syncthreads();
+        const int n_list = *flag;
+        const int n_steps = (int)(((long long)n_list * p.map.block_size + kInt4StepTokens - 1) / kInt4StepTokens);
+        const int s0 = (int)((long long)n_steps * share / p.workers), s1 = (int)((long long)n_steps * (share + 1) / p.workers);
+        float* base = p.parts + (long long)item * p.workers * state;
+        run_item<D, NT, ROWS, LIST>(p, sq, b, R, 0, s0, s1, p.workers == 1, base + share * state, base, base + state, state, p.workers,
+                                    p.counters + item, list, n_list, lds, flag, wave, lane);
+    } else {
+        const int T = p.map.T, B = p.map.B;
+        if (p.zero_rest && p.map.query_start) {           // rows of no sequence
+            const int from = max(0, min(p.map.query_start[B], T)), lead = max(0, min(p.map.query_start[0], T));
+            for (long long r = blockIdx.x; r < lead + (long long)(T - from); r += gridDim.x) {
+                const long long t = r < lead ? r : from + (r - lead);
+                for (int e = threadIdx.x * 2; e < p.Hq * D; e += 512) put_out(p, t * p.Hq * D + e, 0.f, 0.f);
+                if (p.lse) for (int e = threadIdx.x; e < p.Hq; e += 256) p.lse[t * p.Hq + e] = -3.4e38f;
+            }
+        }
+        // Consecutive pieces go to workgroups of one XCD (workgroups are dealt to the eight XCDs in turn), so that the row
+        // tiles of a kv head meet its tokens in one L2.
+        const int per = (p.workers + 7) / 8;
+        const int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+        if (w >= p.workers) return;
+        // the line of steps: its length, and where this workgroup's piece begins
+        const bool lanes_b = B >= 16;     // a lane per sequence, or the wave over the row tiles of each
+        long long total = 0;
+        for (int b0 = 0; b0 < B; b0 += lanes_b ? 64 : 1) {
+            if (lanes_b) total += wave_sum(b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0);
+            else total += head_steps_wave(p, seq_of(p.map, b0), lane);
+        }
+        total *= p.Hkv;
+        const long long piece = max((long long)p.min_steps, (total + p.workers - 1) / p.workers);
+        long long g = (long long)w * piece;
+        const long long g1 = min(total, g + piece);
+        if (g >= g1) return;
+        int b = 0;
+        long long off = g, heads = 0;
+        if (lanes_b) {
+            for (int b0 = 0; b0 < B; b0 += 64) {
+                const long long mine = b0 + lane < B ? p.Hkv * head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
+                const long long incl = wave_scan(mine, lane);
+                const unsigned long long past = __ballot(incl > off);
+                if (past) {
+                    const int at = __ffsll(past) - 1;
+                    off -= __shfl(incl - mine, at);
+                    heads = __shfl(mine, at) / p.Hkv;
+                    b = b0 + at;
+                    break;
+                }
+                off -= __shfl(incl, 63);
+            }
+        } else {
+            for (;; ++b) {
+                heads = head_steps_wave(p, seq_of(p.map, b), lane);
+                if (off < heads * p.Hkv) break;
+                off -= heads * p.Hkv;
+            }
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        Seq sq = seq_of(p.map, b);
+        int h = __builtin_amdgcn_readfirstlane((int)(off / heads));
+        off -= h * heads;
+        int rt = 0;
+        if (!p.causal) {
+            rt = (int)(off / steps_of(p, sq, 0));
+            off -= (long long)rt * steps_of(p, sq, 0);
+        } else {
+            const int nt = row_tiles(p, sq);
+            for (int r0 = 0; r0 < nt; r0 += 64) {
+                const long long mine = r0 + lane < nt ? steps_of(p, sq, r0 + lane) : 0;
+                const long long incl = wave_scan(mine, lane);
+                const unsigned long long past = __ballot(incl > off);
+                if (past) {
+                    const int at = __ffsll(past) - 1;
+                    off -= __shfl(incl - mine, at);
+                    rt = r0 + at;
+                    break;
+                }
+                off -= __shfl(incl, 63);
+            }
+        }
+        rt = __builtin_amdgcn_readfirstlane(rt);
+        int s0 = __builtin_amdgcn_readfirstlane((int)off);
+        while (true) {
+            const int n_steps = steps_of(p, sq, rt);
+            const int s1 = (int)min((long long)n_steps, s0 + (g1 - g));
+            const long long item0 = g - s0;
+            const int w0 = (int)(item0 / piece), w1 = (int)((item0 + n_steps - 1) / piece);
+            const Rows R{sq.first, h * p.G, p.G, h, sq.n * p.G};
+            // slot 2 w + 1: the item begins in w's piece; slot 2 w: it began before
+            run_item<D, NT, ROWS, LIST>(p, sq, b, R, rt * p.rows_tile, s0, s1, w0 == w1, p.parts + (2ll * w + (s0 == 0)) * state,
+                                        p.parts + (2ll * w0 + 1) * state, p.parts + 2ll * (w0 + 1) * state, 2 * state, w1 - w0 + 1,
+                                        p.counters + w0, nullptr, 0, lds, flag, wave, lane);
+            g += s1 - s0;
+            if (g >= g1) break;
+            s0 = 0;
+            if (++rt == row_tiles(p, sq)) {
+                rt = 0;
+                if (++h == p.Hkv) {
+                    h = 0;
+                    do sq = seq_of(p.map, ++b); while (sq.n == 0);
+                }
+            }
+        }
+    }
+}
+
+template <int D, int NT, bool ROWS, bool LIST>
+hipError_t launch_one(const Int4AttnParams& p, hipStream_t s, int* resident) {
+    auto kern = int4_attention_kernel<D, NT, ROWS, LIST>;
+    const size_t lds_bytes = (size_t)Lds<D, NT, ROWS, LIST>::fixed + (LIST ? (size_t)p.P * sizeof(int2) : 0);
+    static int lds_limit[kMaxDevices];
+    hipError_t e = ensure_lds_limit((const void*)kern, lds_limit, lds_bytes);
+    if (e != hipSuccess) return e;
+    if (resident) {
+        static int seen[kMaxDevices];     // (the lists' kernels are not resident grids: asked with the smallest list)
+        static std::mutex seen_mutex;
+        int dev = 0, occ = 0;
+        e = hipGetDevice(&dev);
+        if (e != hipSuccess) return e;
+        if (dev < 0 || dev >= kMaxDevices) return hipErrorInvalidDevice;
+        std::lock_guard<std::mutex> lock(seen_mutex);
+        if (seen[dev] == 0) {
+            e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, 256, (size_t)Lds<D, NT, ROWS, LIST>::fixed);
+            if (e != hipSuccess) return e;
+            seen[dev] = (occ < 1 ? 1 : occ) * device_cu_count();
+        }
+        *resident = seen[dev];
+        return hipSuccess;
+    }
+    const unsigned grid = LIST ? (unsigned)(p.map.B * p.list_rows * p.workers) : (unsigned)((p.workers + 7) / 8 * 8);
+    if (grid == 0) return hipSuccess;
+    count_launch();
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds_bytes, s, p);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t dispatch(const Int4AttnParams& p, hipStream_t s, int* resident) {
+    if (p.lists) {
+        if (p.nt == 1) return launch_one<D, 1, false, true>(p, s, resident);
+        if constexpr (D <= 128) if (p.nt == 4) return launch_one<D, 4, false, true>(p, s, resident);
+        return p.nt == 2 ? launch_one<D, 2, false, true>(p, s, resident) : hipErrorInvalidConfiguration;
+    }
+    if (p.by_rows) return p.nt == 2 ? launch_one<D, 2, true, false>(p, s, resident) : hipErrorInvalidConfiguration;
+    if (p.nt == 1) return launch_one<D, 1, false, false>(p, s, resident);
+    if constexpr (D <= 128) if (p.nt == 4) return launch_one<D, 4, false, false>(p, s, resident);
+    return p.nt == 2 ? launch_one<D, 2, false, false>(p, s, resident) : hipErrorInvalidConfiguration;
+}
+hipError_t any_launch(const Int4AttnParams& p, hipStream_t s, int* resident) {
+    switch (p.D) {
+        case 32: return dispatch<32>(p, s, resident);
+        case 64: return dispatch<64>(p, s, resident);
+        case 128: return dispatch<128>(p, s, resident);
+        case 256: return dispatch<256>(p, s, resident);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_int4_attention(const Int4AttnParams& p, hipStream_t s) { return any_launch(p, s, nullptr); }
+int int4_attention_resident(const Int4AttnParams& p) {
+    int n = 0;
+    if (device_cu_count() <= 0 || any_launch(p, nullptr, &n) != hipSuccess) { (void)hipGetLastError(); return 0; }
+    return n;
+}
+
+}  // namespace spfa

@@ -14,7 +14,7 @@ constexpr int kThreads = 256;           // 4 wave64 per workgroup
 constexpr int kCentWaves = 8;           // waves per workgroup of the standalone scoring kernels: one q row each after
                                         // the shared centroid pass (8 rows per pass at C = 2048)
 
-enum DType : int { kF16 = 0, kBF16 = 1, kI8 = 2, kF32 = 3 };
+enum DType : int { kF16 = 0, kBF16 = 1, kI8 = 2, kF32 = 3, kI4 = 4 };   // kI4: two codes a byte (4-bit caches)
 
 // ComputeCent / CentSelect (no attention).  One workgroup per (group of sequences, kv head).
 struct CentParams {
@@ -60,9 +60,10 @@ struct SelectParams {
 
 // AssignBlockIds: cluster ids of newly filled KV pages.  One workgroup per (kv head, group of rows_per_pass new pages).
 struct AssignParams {
-    const void* kcache;        // BSH [blocks, bs, Hkv, D] | BNSD [blocks, Hkv, bs, D]
+    const void* kcache;        // BSH [blocks, bs, Hkv, D] | BNSD [blocks, Hkv, bs, D]; 4 bits: [blocks, Hkv, bs, D / 2]
     long long blk_stride, tok_stride, head_stride;   // bytes
     int kv_dtype, n_blocks;
+    const void* key_params;    // 4-bit K: float16 [blocks, Hkv, bs, 2], scale and zero of every token, else null
     const void* cent;          // [Hkv, C, D] f16 | bf16
     int qk_dtype;              // dtype of the centroids (the page means are rounded to it)
     const void* antiq_scale;   // int8 K: [2, Hkv*D] or [2] in the centroid dtype (key parameters first), else null

@@ -92,6 +92,15 @@ aclnnAssignBlockIdsGetWorkspaceSize = _sig("aclnnAssignBlockIdsGetWorkspaceSize"
                                            [T] * 7 + [c_int64, c_int64, T] + _WS)
 aclnnAssignBlockIds = _sig("aclnnAssignBlockIds", c_int, _EXEC)
 aclnnSparsePagedFusionAttentionNoAlloc = _sig("aclnnSparsePagedFusionAttentionNoAlloc", c_int, [T, c_void_p])
+aclnnAppendKvCacheGetWorkspaceSize = _sig("aclnnAppendKvCacheGetWorkspaceSize", c_int,
+                                          [T] * 10 + [c_int64] * 4 + [T] * 5 + _WS)
+aclnnAppendKvCache = _sig("aclnnAppendKvCache", c_int, _EXEC)
+aclnnGatherKvCacheGetWorkspaceSize = _sig("aclnnGatherKvCacheGetWorkspaceSize", c_int,
+                                          [T] * 9 + [c_int64] * 3 + [T] * 2 + _WS)
+aclnnGatherKvCache = _sig("aclnnGatherKvCache", c_int, _EXEC)
+aclnnPagedAttentionInt4GetWorkspaceSize = _sig("aclnnPagedAttentionInt4GetWorkspaceSize", c_int,
+                                               [T] * 9 + [c_double] + [c_int64] * 5 + [T] * 2 + _WS)
+aclnnPagedAttentionInt4 = _sig("aclnnPagedAttentionInt4", c_int, _EXEC)
 
 
 def describe(executor) -> dict:

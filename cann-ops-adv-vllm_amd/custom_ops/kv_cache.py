@@ -1,0 +1,170 @@
+"""KV-cache operators: what fills the paged cache that the sparse attention ops read, a cache held in 4 bits, and dense
+attention over it.  No counterpart in the reference, whose ops only read the cache (extension/custom_ops/add_custom.py);
+conventions (block_table, seq_len, block_size, antiquant parameters, GPU tensors only, torch's current stream) are those of
+`add_custom`.
+
+Tokens of a call.  Rows query_start[b] .. query_start[b + 1] belong to sequence b (query_start [B + 1] int32 on the GPU;
+None: row b, one per sequence).  The i-th of n rows stands at position seq_len[b] - n + i — seq_len [B] int32 counts the
+sequence with its new rows — and lives in row pos % block_size of page block_table[b][pos // block_size].
+
+The 4-bit cache is four tensors (`empty_int4_cache`): a token of a kv head is D codes and a (scale, zero) pair,
+x = scale * code + zero.
+    key_cache    uint8 [blocks, Hkv, bs, D / 2]         byte i: channel 2 i (low bits), channel 2 i + 1 (high bits)
+    value_cache  uint8 [blocks, Hkv, bs / 4, D / 2, 4]  the same bytes, those of four consecutive tokens side by side
+    key_params, value_params  float16 [blocks, Hkv, bs, 2]
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _abi
+from .add_custom import _destroy
+
+
+class Int4Cache(NamedTuple):
+    key_cache: torch.Tensor
+    value_cache: torch.Tensor
+    key_params: torch.Tensor
+    value_params: torch.Tensor
+
+
+def empty_int4_cache(num_blocks: int, num_key_value_heads: int, block_size: int, head_dim: int, device="cuda") -> Int4Cache:
+    """The tensors of a 4-bit cache, zeroed (every token reads as zeros)."""
+    if block_size <= 0 or block_size % 16 or head_dim not in (32, 64, 128, 256):
+        raise _abi.AclError("a 4-bit cache needs a block size that is a multiple of 16 and a head dim of 32, 64, 128 or 256")
+    n, h, bs, d = int(num_blocks), int(num_key_value_heads), int(block_size), int(head_dim)
+    zeros = lambda shape, dt: torch.zeros(shape, dtype=dt, device=device)   # noqa: E731
+    return Int4Cache(zeros((n, h, bs, d // 2), torch.uint8), zeros((n, h, bs // 4, d // 2, 4), torch.uint8),
+                     zeros((n, h, bs, 2), torch.float16), zeros((n, h, bs, 2), torch.float16))
+
+
+def _one_device(what, *tensors):
+    """All operands on the GPU, and on the same one (they reach the kernel as bare addresses)."""
+    _abi.require_gpu(*tensors)
+    devs = {t.device for t in tensors if isinstance(t, torch.Tensor) and t.numel() > 0}
+    if len(devs) > 1:
+        raise _abi.AclError(f"{what}: operands on several devices {sorted(map(str, devs))}")
+
+
+def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                    block_table: torch.Tensor, seq_len: torch.Tensor, *, query: Optional[torch.Tensor] = None,
+                    query_out: Optional[torch.Tensor] = None, query_start: Optional[torch.Tensor] = None,
+                    cos_sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                    interleaved: bool = False, block_size: int = 128, antiquant_scale: Optional[torch.Tensor] = None,
+                    antiquant_offset: Optional[torch.Tensor] = None, antiquant_mode: int = 0,
+                    key_params: Optional[torch.Tensor] = None, value_params: Optional[torch.Tensor] = None
+                    ) -> Optional[torch.Tensor]:
+    """Write the new rows key, value [T, Hkv, D] (float16 / bfloat16, any token and head stride) into the paged cache,
+    rotated by position on the way; query [T, Hq, D] is rotated along and returned (None without query).  One launch.
+
+    cos_sin [rows, R] (float32 or the rows' dtype): R / 2 cosines, then R / 2 sines of a position; the channel pairs
+    (i, i + R / 2) — (2 i, 2 i + 1) with interleaved — of q and K turn by them, channels from R on pass through.  positions
+    [T] int32 names the table rows (default: the position in the sequence).  No cos_sin: no rotation.
+
+    The caches have the rows' dtype ([blocks, bs, Hkv * D], [blocks, bs, Hkv, D] or [blocks, Hkv, bs, D]), are int8 in the
+    same shapes (antiquant_scale / antiquant_offset as the attention ops take them, modes 0 and 2) or uint8: 4 bits, with
+    key_params / value_params.  query_out may be query itself; where it is given, rows in no sequence are left as they are
+    (a new tensor holds zeros there)."""
+    _one_device("append_kv_cache", key, value, key_cache, value_cache, block_table, seq_len, query, query_out, query_start, cos_sin,
+                positions, antiquant_scale, antiquant_offset, key_params, value_params)
+    own_out = query is not None and query_out is None
+    if query is None and query_out is not None:
+        raise _abi.AclError("append_kv_cache: query_out given without query")
+    if own_out:
+        query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if key.dim() == 3 and key.shape[0] == 0:
+        return query_out                                     # no rows
+    descs = [_abi.to_acl(t) for t in (key, value, query, cos_sin, positions, block_table, seq_len, query_start, antiquant_scale,
+                                      antiquant_offset)]
+    outs = [_abi.to_acl(t) for t in (key_cache, value_cache, key_params, value_params, query_out)]
+    try:
+        _abi.run(_abi.aclnnAppendKvCacheGetWorkspaceSize, _abi.aclnnAppendKvCache,
+                 descs + [int(block_size), int(bool(interleaved)), int(antiquant_mode), int(own_out)] + outs, key.device,
+                 "aclnnAppendKvCache")
+    finally:
+        _destroy(descs + outs)
+    return query_out
+
+
+def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
+                    num_key_value_heads: int, *, query_start: Optional[torch.Tensor] = None, num_tokens: Optional[int] = None,
+                    block_size: int = 128, antiquant_scale: Optional[torch.Tensor] = None,
+                    antiquant_offset: Optional[torch.Tensor] = None, antiquant_mode: int = 0,
+                    key_params: Optional[torch.Tensor] = None, value_params: Optional[torch.Tensor] = None,
+                    out_dtype: Optional[torch.dtype] = None, key_out: Optional[torch.Tensor] = None,
+                    value_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The last rows of every sequence (query_start; None: the last one) out of a paged cache of any type, in 16 bits:
+    (K [T, Hkv, D], V).  num_tokens is T (needed with query_start, which lives on the GPU).  Tokens without a place in the
+    cache read as zeros; rows in no sequence are zeros in new tensors and left as they are in key_out / value_out.
+    out_dtype: float16 or bfloat16 (default: the cache's, the antiquant parameters' or float16)."""
+    _one_device("gather_kv_cache", key_cache, value_cache, block_table, seq_len, query_start, antiquant_scale, antiquant_offset,
+                key_params, value_params, key_out, value_out)
+    if (key_out is None) != (value_out is None):
+        raise _abi.AclError("gather_kv_cache: key_out and value_out come together")
+    own_out = key_out is None
+    if own_out:
+        n = int(num_tokens) if num_tokens is not None else (seq_len.shape[0] if query_start is None else None)
+        if n is None:
+            raise _abi.AclError("gather_kv_cache: num_tokens must be given with query_start")
+        heads = int(num_key_value_heads)
+        if key_cache.dtype == torch.uint8:
+            d = key_cache.shape[-1] * 2
+        else:
+            d = key_cache.shape[-1] if key_cache.dim() == 4 else key_cache.shape[-1] // heads
+        if out_dtype is None:
+            out_dtype = {torch.uint8: torch.float16, torch.int8: getattr(antiquant_scale, "dtype", torch.float16)}.get(
+                key_cache.dtype, key_cache.dtype)
+        key_out = torch.empty((n, heads, d), dtype=out_dtype, device=key_cache.device)
+        value_out = torch.empty_like(key_out)
+    if key_out.shape[0] == 0:
+        return key_out, value_out
+    descs = [_abi.to_acl(t) for t in (key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
+                                      antiquant_scale, antiquant_offset)]
+    outs = [_abi.to_acl(key_out), _abi.to_acl(value_out)]
+    try:
+        _abi.run(_abi.aclnnGatherKvCacheGetWorkspaceSize, _abi.aclnnGatherKvCache,
+                 descs + [int(block_size), int(antiquant_mode), int(own_out)] + outs, key_cache.device, "aclnnGatherKvCache")
+    finally:
+        _destroy(descs + outs)
+    return key_out, value_out
+
+
+def paged_attention_int4(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, key_params: torch.Tensor,
+                         value_params: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor, scale_value: float,
+                         num_key_value_heads: int, *, query_start: Optional[torch.Tensor] = None,
+                         max_query_len: Optional[int] = None, causal: bool = True,
+                         block_position: Optional[torch.Tensor] = None, block_size: int = 128,
+                         softmax_lse: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                         out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Attention of query [T, Hq, D] over a 4-bit cache; returns [T, Hq, D] in query's dtype (out_dtype=torch.float32: not
+    rounded).  One launch.
+
+    query_start None: decode, one row per sequence.  With query_start: several rows per sequence (candidate tokens, prompt
+    chunks; append_kv_cache has stored their K and V), max_query_len the most rows of one sequence (default T; an upper bound
+    is fine).  causal: a row sees the tokens up to its own position; False: all seq_len[b] tokens (an encoder's states).
+    block_position [B, Hq | Hkv, P] int32 (decode only): the logical pages each row attends, as cent_select returns them.
+    softmax_lse: float32 [T, Hq], filled with the rows' log-sum-exp.  A row that sees no token is zero; rows in no sequence
+    are zero in a new tensor and left as they are in `out`."""
+    _one_device("paged_attention_int4", query, key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
+                block_position, softmax_lse, out)
+    own_out = out is None
+    if own_out:
+        out = torch.empty(query.shape, dtype=out_dtype or query.dtype, device=query.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise _abi.AclError("paged_attention_int4: out and out_dtype disagree")
+    if query.dim() == 3 and query.shape[0] == 0:
+        return out
+    if max_query_len is None:
+        max_query_len = query.shape[0]
+    descs = [_abi.to_acl(t) for t in (query, key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
+                                      block_position)]
+    outs = [_abi.to_acl(out), _abi.to_acl(softmax_lse)]
+    try:
+        _abi.run(_abi.aclnnPagedAttentionInt4GetWorkspaceSize, _abi.aclnnPagedAttentionInt4,
+                 descs + [float(scale_value), int(num_key_value_heads), int(block_size), int(max_query_len), int(bool(causal)),
+                          int(own_out)] + outs, query.device, "aclnnPagedAttentionInt4")
+    finally:
+        _destroy(descs + outs)
+    return out
