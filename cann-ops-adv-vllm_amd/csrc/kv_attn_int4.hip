@@ -1,7 +1,8 @@
 // Attention over a paged cache held in 4 bits (gfx950).
 //
 //   K_t = s_t c_t + z_t,  V_t = s'_t c'_t + z'_t    (codes c, c' in 0 .. 15; s, z per token and kv head, float16)
-//   score(n, t) = scale (s_t (q_n . c_t) + z_t sum(q_n)),   O_n = (sum_t (p_t s'_t) c'_t + sum_t p_t z'_t) / sum_t p_t
+//   score(n, t) = scale (s_t (q_n . c_t) + z_t sum(q_n)),
+//   O_n = (sum_t (p_t s'_t) (c'_t - 7.5) + sum_t p_t (z'_t + 7.5 s'_t)) / sum_t p_t
 //
 // so the matrix cores multiply CODES and the parameters are applied to scores and probabilities, one fma each.  A code
 // becomes a matrix operand by masking alone: (w & 0x000f000f) are two codes in the bits of float16 denormals c * 2^-24
@@ -22,8 +23,9 @@
 // form one line that is cut into equal pieces, one per resident workgroup: lengths may be as ragged as they like.  A
 // workgroup computes its piece from seq_len alone.  An item that spans several workgroups is merged by the last of them
 // to arrive (partial states in the workspace, one arrival counter per split item).
-//   by tokens (few rows): the four waves of a workgroup take every fourth step, states merged through LDS;
-//   by rows (prompts): the four waves hold different rows and walk the same tokens (shared through the L1 cache).
+// The four waves of a workgroup are RW groups of rows x 4 / RW shares of the steps: few rows (decode) share the steps and
+// merge their states through LDS, prompts hold four times as many rows and walk the same tokens (shared through the L1
+// cache), candidate tokens are in between.
 // With page lists (one row of q per sequence) an item is (sequence, list) and workers workgroups share each list.
 #include "kv_params.h"
 
@@ -39,6 +41,7 @@ namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;          // reference of a row that has seen no token
@@ -50,16 +53,21 @@ constexpr int kScaleTop = 6;                // V scales are brought below 2^6 (a
 struct Ptrs { int phys[2], row[2], tok[2]; };
 
 template <int W> struct Words { uint32_t w[W]; };
-template <int W>
+// STREAM: bytes that nobody reads again soon (decode): 268 -> 250 us for 1.4 GB against ordinary loads
+template <int W, bool STREAM>
 __device__ __forceinline__ Words<W> load_words(const uint8_t* p) {
+    auto ld = [](auto* a) {
+        if constexpr (STREAM) return __builtin_nontemporal_load(a);
+        else return *a;
+    };
     Words<W> r;
-    if constexpr (W == 1) r.w[0] = *(const uint32_t*)p;
-    else if constexpr (W == 2) { const uint2 v = *(const uint2*)p; r.w[0] = v.x; r.w[1] = v.y; }
+    if constexpr (W == 1) r.w[0] = ld((const uint32_t*)p);
+    else if constexpr (W == 2) { const u32x2 v = ld((const u32x2*)p); r.w[0] = v[0]; r.w[1] = v[1]; }
     else {
 #pragma unroll
         for (int i = 0; i < W / 4; ++i) {
-            const uint4 v = *(const uint4*)(p + 16 * i);
-            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+            const u32x4 v = ld((const u32x4*)(p + 16 * i));
+            r.w[4 * i] = v[0]; r.w[4 * i + 1] = v[1]; r.w[4 * i + 2] = v[2]; r.w[4 * i + 3] = v[3];
         }
     }
     return r;
@@ -95,6 +103,15 @@ __device__ __forceinline__ Seq seq_of(const TokenMap& m, int b) {
     s.tokens = max(m.seq_len[b], 0);
     s.len = (int)min((long long)s.tokens, (long long)m.max_page * m.block_size);
     return s;
+}
+// The same values, known to be the same in all lanes (they then live in scalar registers).
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uni(long long x) {
+    return (long long)(((unsigned long long)(unsigned)uni((int)((unsigned long long)x >> 32)) << 32) | (unsigned)uni((int)x));
+}
+__device__ __forceinline__ Seq uniform_seq(const TokenMap& m, int b) {
+    const Seq s = seq_of(m, b);
+    return Seq{uni(s.first), uni(s.n), uni(s.tokens), uni(s.len)};
 }
 // Tokens that row i of a sequence sees: its position is seq_len - n + i, and nothing lies behind the table.
 __device__ __forceinline__ int seen_by(const Int4AttnParams& p, const Seq& s, int i) {
@@ -138,6 +155,7 @@ __device__ __forceinline__ long long head_steps_wave(const Int4AttnParams& p, co
 template <int D, int NT>
 struct State {
     f32x4 o[NT][D / 16];     // [2 j + parity][i]: channel (4 kg + i) * D / 16 + 2 j + parity, in units of the codes
+    f32x4 r[NT];             // sum of w (every element holds it)
     float m[NT], l[NT], z[NT];
     float inv_r;             // power of two: V scales are taken times inv_r
     int seen;                // bit t: the lane's row of tile t has seen a token
@@ -148,6 +166,7 @@ __device__ __forceinline__ void clear_state(State<D, NT>& S) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         S.m[t] = S.l[t] = S.z[t] = 0.f;
+        S.r[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) S.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -173,40 +192,51 @@ struct Rows { int first, head0, G, kvh, n; };
 // float16's range included), and the even slots, 16 times larger, stay below 2^15.
 template <int D, int NT>
 __device__ __forceinline__ void load_query(const Int4AttnParams& p, const Seq& s, const Rows& R, int row0, Query<D, NT>& Q, int lane) {
-    constexpr int W = D / 32, E = 8 * W;      // words / channels of a lane
+    constexpr int W = D / 32;                 // 16-byte pieces (8 channels) of a lane
     const int n = lane & 15, kg = lane >> 4;
     const bool bf = p.q_dtype == kBF16;
-    uint32_t raw[NT][E / 2];
+    // eight channels of the lane's row of tile t
+    auto piece = [&](int t, int j, float (&x)[8]) {
+        const int r = row0 + 16 * t + n;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (r < R.n) {
+            const int i = r / R.G;
+            const uint16_t* src = (const uint16_t*)p.q + (long long)(R.first + i) * p.q_tok + (long long)(R.head0 + r - i * R.G) * p.q_head +
+                                  kg * 8 * W + 8 * j;
+            if (p.q_wide) {
+                const uint4 v = *(const uint4*)src;
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = bf ? bf16_lo(w[e]) : lo16(w[e]);
+            x[2 * e + 1] = bf ? bf16_hi(w[e]) : hi16(w[e]);
+        }
+    };
     float top = 0.f;
     Q.lim_min = 0x7fffffff;
     Q.lim_max = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 16 * t + n;
-        const bool live = r < R.n;
-        const int i = live ? r / R.G : 0, g = live ? r - i * R.G : 0;
-        const uint16_t* src = (const uint16_t*)p.q + (long long)(R.first + i) * p.q_tok + (long long)(R.head0 + g) * p.q_head + kg * E;
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) raw[t][e] = 0u;
-        if (live && p.q_wide) {
+        for (int j = 0; j < W; ++j) {
+            float x[8];
+            piece(t, j, x);
 #pragma unroll
-            for (int e = 0; e < E / 8; ++e) {
-                const uint4 v = *(const uint4*)(src + 8 * e);
-                raw[t][4 * e] = v.x; raw[t][4 * e + 1] = v.y; raw[t][4 * e + 2] = v.z; raw[t][4 * e + 3] = v.w;
+            for (int e = 0; e < 8; ++e) {
+                sum += x[e];
+                top = fmaxf(top, fabsf(x[e]));
             }
-        } else if (live) {
-#pragma unroll
-            for (int e = 0; e < E / 2; ++e) raw[t][e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
-        }
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-            const float a = bf ? bf16_lo(raw[t][e]) : lo16(raw[t][e]), b = bf ? bf16_hi(raw[t][e]) : hi16(raw[t][e]);
-            sum += a + b;
-            top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
         }
         Q.sum[t] = rows_sum(sum) * (p.scale * kLog2e);
-        Q.lim[t] = live ? seen_by(p, s, i) : 0;
+        const int r = row0 + 16 * t + n;
+        const bool live = r < R.n;
+        Q.lim[t] = live ? seen_by(p, s, r / R.G) : 0;
         if (live) {
             Q.lim_min = min(Q.lim_min, Q.lim[t]);
             Q.lim_max = max(Q.lim_max, Q.lim[t]);
@@ -217,156 +247,174 @@ __device__ __forceinline__ void load_query(const Int4AttnParams& p, const Seq& s
         Q.lim_min = min(Q.lim_min, __shfl_xor(Q.lim_min, d));
         Q.lim_max = max(Q.lim_max, __shfl_xor(Q.lim_max, d));
     }
-    Q.lim_min = __builtin_amdgcn_readfirstlane(Q.lim_min);
-    Q.lim_max = __builtin_amdgcn_readfirstlane(Q.lim_max);
+    Q.lim_min = uni(Q.lim_min);
+    Q.lim_max = uni(Q.lim_max);
     // exponent of the largest element (an infinite query is not scaled: its row comes out NaN)
     const int eb = (int)((__float_as_uint(top) >> 23) & 255u);
-    int up = (top > 0.f && eb < 255) ? 127 + 10 - eb : 0;
-    up = __builtin_amdgcn_readfirstlane(max(-118, min(118, up)));
+    const int up = uni(max(-118, min(118, (top > 0.f && eb < 255) ? 127 + 10 - eb : 0)));
     const float f = __uint_as_float((uint32_t)(127 + up) << 23);
     // codes arrive as c * 2^-24 (even channels) and 16 c * 2^-24 (odd); even slots of q carry 16 f, odd ones f
     Q.ks = p.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;   // 2^24 / 16
+    // (the rows are read again, from the cache, rather than kept: they would take the registers of the sums to come)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < W; ++j) {
             float x[8];
+            piece(t, j, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = raw[t][4 * j + e];
-                x[2 * e] = (bf ? bf16_lo(w) : lo16(w)) * (16.f * f);
-                x[2 * e + 1] = (bf ? bf16_hi(w) : hi16(w)) * f;
-            }
+            for (int e = 0; e < 8; ++e) x[e] *= (e & 1) ? f : 16.f * f;
             Q.q[t][j] = u32x4{pack_f16(x[0], x[4]), pack_f16(x[1], x[5]), pack_f16(x[2], x[6]), pack_f16(x[3], x[7])};
         }
 }
 
-// The data of one step.
+// The data of one step: the codes of both halves, and one parameter pair per lane (lanes 0 .. 31 the K pairs of the 32
+// tokens, lanes 32 .. 63 the V pairs), which go through LDS to the lanes that need them: one load and one register for
+// what as operands takes sixteen.
 template <int D>
 struct Tile {
     Words<D / 32> k[2], v[2];
-    u32x4 kp[2], vp[2];
+    uint32_t par;
 };
-
-template <int D>
+// First row of a half step in the codes and parameters: row index over the whole cache.
+__device__ __forceinline__ long long row_at(const Int4AttnParams& p, int kvh, const Ptrs& a, int i) {
+    return ((long long)max(a.phys[i], 0) * p.Hkv + kvh) * p.map.block_size + a.row[i];
+}
+template <int D, bool STREAM>
 __device__ __forceinline__ void load_tile(const Int4AttnParams& p, int kvh, const Ptrs& a, Tile<D>& t, int lane) {
-    constexpr int W = D / 32;
-    const int n = lane & 15, kg = lane >> 4;
+    const long long r0 = row_at(p, kvh, a, 0), r1 = row_at(p, kvh, a, 1);
+    const long long rp = (lane & 16) ? r1 : r0;
+    t.par = (lane < 32 ? p.k_params : p.v_params)[rp + (lane & 15)];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const long long row = ((long long)max(a.phys[i], 0) * p.Hkv + kvh) * p.map.block_size + a.row[i];
-        const uint8_t* kb = p.kcache + row * (D / 2);
-        const uint8_t* vb = p.vcache + row * (D / 2);
-        t.k[i] = load_words<W>(kb + (unsigned)(n * (D / 2) + kg * 4 * W));
-        t.v[i] = load_words<W>(vb + (unsigned)(kg * (D / 2 * 4) + n * 4 * W));
-        t.kp[i] = *(const u32x4*)((const uint8_t*)(p.k_params + row) + (unsigned)(kg * 16));
-        t.vp[i] = *(const u32x4*)((const uint8_t*)(p.v_params + row) + (unsigned)(kg * 16));
+        const long long row = i ? r1 : r0;
+        t.k[i] = load_words<D / 32, STREAM>(p.kcache + row * (D / 2) + (unsigned)((lane & 15) * (D / 2) + (lane >> 4) * (D / 8)));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const long long row = i ? r1 : r0;
+        t.v[i] = load_words<D / 32, STREAM>(p.vcache + row * (D / 2) + (unsigned)((lane >> 4) * (2 * D) + (lane & 15) * (D / 8)));
     }
 }
+struct Params { u32x4 k[2], v[2]; };     // of the lane's four tokens in each half
+__device__ __forceinline__ Params spread_params(uint32_t par, uint32_t* stage, int lane) {
+    wave_lds_sync();                     // (the reads of the step before are done)
+    stage[lane] = par;
+    wave_lds_sync();
+    const u32x4* at = (const u32x4*)(stage + (lane >> 4) * 4);
+    return Params{{at[0], at[4]}, {at[8], at[12]}};
+}
 
-// One step of a wave.  MASKED: some token of the step is hidden from some row (the end of the sequence, the causal
+// A step in three parts.  MASKED: some token of the step is hidden from some row (the end of the sequence, the causal
 // border, a page that is not there); a hidden token counts as probability 0 whatever its parameters hold.
-template <int D, int NT, bool MASKED>
-__device__ __forceinline__ void attend(const Query<D, NT>& Q, State<D, NT>& S, const Tile<D>& T, const Ptrs& a, int seq_end, int lane) {
-    constexpr int W = D / 32;
-    const int kg = lane >> 4;
-    f32x4 s[2][NT];
+template <int D, int NT>
+__device__ __forceinline__ void products(const Query<D, NT>& Q, const Tile<D>& T, f32x4 (&s)[2][NT]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
+        for (int j = 0; j < D / 32; ++j) {
             const u32x4 c = codes_of(T.k[i].w[j]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[i][t] = mfma(c, Q.q[t][j], s[i][t]);
         }
     }
-    float vs[2][4], vs_top = 0.f;
+}
+// scores relative to the rows' references (log2), largest of them
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ float scores(const Query<D, NT>& Q, const State<D, NT>& S, const Params& P, const Ptrs& a, int seq_end, int kg,
+                                        f32x4 (&s)[2][NT]) {
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int tok = a.tok[i] + 4 * kg + e;
-            const bool there = !MASKED || (a.phys[i] >= 0 && tok < seq_end);
-            vs[i][e] = there ? lo16(T.vp[i][e]) * S.inv_r : 0.f;
-            vs_top = fmaxf(vs_top, vs[i][e]);
-        }
-    // scores relative to the rows' references (log2)
-    float x_top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float ks = lo16(T.kp[i][e]) * Q.ks, kz = hi16(T.kp[i][e]);
+            const float ks = lo16(P.k[i][e]) * Q.ks, kz = hi16(P.k[i][e]);
             const int tok = a.tok[i] + 4 * kg + e;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float x = fmaf(s[i][t][e], ks, fmaf(kz, Q.sum[t], -S.m[t]));
                 if (MASKED && (a.phys[i] < 0 || tok >= min(seq_end, Q.lim[t]))) x = -__builtin_inff();
                 s[i][t][e] = x;
-                x_top = fmaxf(x_top, x);
+                top = fmaxf(top, x);
             }
         }
-    if (MASKED || S.open || __any(x_top > kLazy || vs_top > (float)(2 << kScaleTop))) {
-        // move the references: rows to their true maxima, the scale reference where it is free or outgrown
-        float vmax = fminf(vs_top, 3.0e38f);
-        for (int d = 1; d < 64; d <<= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, d));
-        float r = 1.f;
-        if (vmax > (float)(2 << kScaleTop) || ((S.open & 2) && vmax > 0.f)) {
-            const int e = max(-60, min(60, (int)((__float_as_uint(vmax) >> 23) & 255u) - 127 + 1 - kScaleTop));
-            r = __uint_as_float((uint32_t)(127 - e) << 23);   // vmax * r in [2^5, 2^6)
-            S.open &= 1;
-        }
-        S.inv_r *= r;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vs[i][e] *= r;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][t][e]);
-            top = rows_max(top);
-            const bool before = (S.seen >> t) & 1, now = top > -__builtin_inff();
-            const float up = before ? fmaxf(top, 0.f) : (now ? top : 0.f);
-            const float alpha = before ? fast_exp2(-up) : 1.f;      // (nothing is in the sums before the first token)
-            S.m[t] += up;
-            S.l[t] *= alpha;
-            S.z[t] *= alpha;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) S.o[t][d] *= alpha * r;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][t][e] -= up;
-            if (now) S.seen |= 1 << t;
-        }
-        const int none = __any(S.seen != (1 << NT) - 1) ? 1 : 0;
-        S.open = __builtin_amdgcn_readfirstlane((S.open & 2) | none);
+    return top;
+}
+// The slow path: rows' references to their true maxima, the scale reference where it is free or outgrown.
+template <int D, int NT>
+__device__ __forceinline__ void move_references(State<D, NT>& S, f32x4 (&s)[2][NT], float (&vs)[2][4], float vs_top) {
+    float vmax = fminf(vs_top, 3.0e38f);
+    for (int d = 1; d < 64; d <<= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, d));
+    float r = 1.f;
+    if (vmax > (float)(2 << kScaleTop) || ((S.open & 2) && vmax > 0.f)) {
+        const int e = max(-60, min(60, (int)((__float_as_uint(vmax) >> 23) & 255u) - 127 + 1 - kScaleTop));
+        r = __uint_as_float((uint32_t)(127 - e) << 23);   // vmax * r in [2^5, 2^6)
+        S.open &= 1;
     }
-    // probabilities; P^T operand: tokens (0, 2), (1, 3) of the lane's four, first half then second half
-    u32x4 pb[NT];
+    S.inv_r *= r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vs[i][e] *= r;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float w[2][4];
+        float top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = s[i][t][e], pr = fast_exp2(x), vz = hi16(T.vp[i][e]);
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][t][e]);
+        top = rows_max(top);
+        const bool before = (S.seen >> t) & 1, now = top > -__builtin_inff();
+        const float up = before ? fmaxf(top, 0.f) : (now ? top : 0.f);
+        const float alpha = before ? fast_exp2(-up) : 1.f;      // (nothing is in the sums before the first token)
+        S.m[t] += up;
+        S.l[t] *= alpha;
+        S.z[t] *= alpha;
+        S.r[t] *= alpha * r;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) S.o[t][d] *= alpha * r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][t][e] -= up;
+        if (now) S.seen |= 1 << t;
+    }
+    const int none = __any(S.seen != (1 << NT) - 1) ? 1 : 0;
+    S.open = __builtin_amdgcn_readfirstlane((S.open & 2) | none);
+}
+// probabilities into the sums and into operand B of the second product: tokens (0, 2), (1, 3) of the lane's four, first
+// half then second half
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ void weights(State<D, NT>& S, const Params& P, const f32x4 (&s)[2][NT], const float (&vs)[2][4], u32x4 (&pb)[NT]) {
+    float w[NT][2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float vz = fmaf(7.5f, lo16(P.v[i][e]), hi16(P.v[i][e]));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float x = s[i][t][e], pr = fast_exp2(x);
                 const bool hidden = MASKED && x == -__builtin_inff();
                 S.l[t] += pr;
                 S.z[t] = hidden ? S.z[t] : fmaf(pr, vz, S.z[t]);
-                w[i][e] = hidden ? 0.f : pr * vs[i][e];
+                w[t][i][e] = hidden ? 0.f : pr * vs[i][e];
             }
-        pb[t] = u32x4{pack_f16(w[0][0], w[0][2]), pack_f16(w[0][1], w[0][3]), pack_f16(w[1][0], w[1][2]), pack_f16(w[1][1], w[1][3])};
-    }
+        }
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
+    for (int t = 0; t < NT; ++t)
+        pb[t] = u32x4{pack_f16(w[t][0][0], w[t][0][2]), pack_f16(w[t][0][1], w[t][0][3]), pack_f16(w[t][1][0], w[t][1][2]),
+                      pack_f16(w[t][1][1], w[t][1][3])};
+}
+template <int D, int NT>
+__device__ __forceinline__ void accumulate(State<D, NT>& S, const Tile<D>& T, const u32x4 (&pb)[NT]) {
+    const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+    for (int t = 0; t < NT; ++t) S.r[t] = mfma(ones, pb[t], S.r[t]);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
         const u32x4 c0 = codes_of(T.v[0].w[j]), c1 = codes_of(T.v[1].w[j]);
         const u32x4 even = {c0[0], c0[2], c1[0], c1[2]}, odd = {c0[1], c0[3], c1[1], c1[3]};
 #pragma unroll
@@ -382,11 +430,11 @@ __device__ __forceinline__ void attend(const Query<D, NT>& Q, State<D, NT>& S, c
 // In registers of a wave: State with o in real units and m, l complete in every lane of the row.
 template <int D, int NT>
 __device__ __forceinline__ void settle(State<D, NT>& S) {
-    const float even = 16777216.f / S.inv_r, odd = even * 0.0625f;
+    const float even = 16777216.f / S.inv_r, odd = even * 0.0625f, mid = 7.5f / S.inv_r;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         S.l[t] = rows_sum(S.l[t]);
-        const float z = rows_sum(S.z[t]);
+        const float z = rows_sum(S.z[t]) - S.r[t][0] * mid;
         if (!((S.seen >> t) & 1) && !(S.l[t] != S.l[t])) S.m[t] = kNoMax;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
@@ -553,105 +601,141 @@ __device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows&
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------
-template <int D, int NT, bool ROWS, bool LIST>
+template <int D, int NT, int RW, bool LIST>
 struct Lds {
-    static constexpr int merge = ROWS ? 0 : 2 * 16 * NT * (D + 2) * 4;
+    static constexpr int merge = RW == 4 ? 0 : 2 * 16 * NT * (D + 2) * 4;   // two states
     static constexpr int join = (1024 / D) * (D + 2) * 4;
-    static constexpr int fixed = (merge > join ? merge : join) + 16;
+    static constexpr int head = (merge > join ? merge : join);
+    static constexpr int fixed = head + 16 + 1024;   // the flag, 256 bytes of parameters per wave
 };
+// Steps whose data is under way, and waves per SIMD that the registers of a variant are cut for.
+#ifndef KV_DEPTH1
+#define KV_DEPTH1 3
+#endif
+template <int D, int NT, int RW, bool LIST> constexpr int depth() { return RW == 1 && NT * D <= 128 && !LIST ? KV_DEPTH1 : 2; }
 
-// Steps [s0, s1) of an item for this wave (every fourth one from s0 + wave, or all of them with ROWS).
-template <int D, int NT, bool ROWS, bool LIST>
+
+// Steps [s0, s1) of an item for this wave: every (4 / RW)-th one from s0 + wave / RW.  The data of DEPTH
+// steps is in registers or on its way: a step's buffer is loaded again as soon as the step is done.  The loads are not
+// conditional (behind the end the last step is loaded again, from the cache), so that the waits between them stay exact.
+template <int D, int NT, int RW, bool LIST>
 __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, const Query<D, NT>& Q, State<D, NT>& S,
-                                     int s0, int s1, const int2* list, int n_list, int wave, int lane) {
-    const int stride = ROWS ? 1 : 4;
-    const int seq_end = sq.len;
-    int s = ROWS ? s0 : s0 + wave;
+                                     int s0, int s1, const int2* list, int n_list, uint32_t* stage, int wave, int lane) {
+    constexpr int stride = 4 / RW, DEPTH = depth<D, NT, RW, LIST>();
+    const int seq_end = sq.len, kg = lane >> 4;
+    int s = s0 + wave / RW;
     // no row of the wave sees anything from lim_max on (lists are not ordered by position: all of theirs is walked)
     if (!LIST) s1 = min(s1, (min(Q.lim_max, seq_end) + kInt4StepTokens - 1) / kInt4StepTokens);
     if (s >= s1) return;
+    const int last = s + (s1 - 1 - s) / stride * stride;
     const int32_t* table = p.map.block_table + (long long)b * p.map.max_page;
     const int bs = p.map.block_size;
-    // page and row of 16 tokens: (units of 16) * ceil(2^32 / (bs / 16)) >> 32, exact below 2^22 units
+    // page of 16 tokens: (units of 16) * ceil(2^32 / (bs / 16)) >> 32, exact below 2^22 units
+    auto page_of = [&](unsigned u) { return (int)(p.page_magic ? __umulhi(u, p.page_magic) : u); };
+    // 64 table entries in one register, the 64 after them in another: a lookup is a lane read
+    int base = page_of(2u * (unsigned)s), cur = 0, nxt = 0;
+    auto entries = [&](int from) { return from + lane < p.map.max_page ? table[from + lane] : -1; };
+    if (!LIST) {
+        cur = entries(base);
+        nxt = entries(base + 64);
+    }
     auto locate = [&](int step, Ptrs& a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const unsigned u = 2u * (unsigned)step + i;
-            const int page = (int)(p.page_magic ? __umulhi(u, p.page_magic) : u);
+            const int page = page_of(u);
             a.row[i] = (int)(16u * u) - page * bs;
+            int e;
             if (LIST) {
-                const int2 e = page < n_list ? list[page] : make_int2(0, -1);
-                a.tok[i] = __builtin_amdgcn_readfirstlane(e.x) * bs + a.row[i];
-                a.phys[i] = e.y;
+                const int2 le = page < n_list ? list[page] : make_int2(0, -1);
+                a.tok[i] = uni(le.x) * bs + a.row[i];
+                e = uni(le.y);
             } else {
                 a.tok[i] = (int)(16u * u);
-                a.phys[i] = a.tok[i] < seq_end ? table[page] : -1;
+                while (page - base >= 64) {
+                    cur = nxt;
+                    base += 64;
+                    nxt = entries(base + 64);
+                }
+                e = a.tok[i] < seq_end ? __builtin_amdgcn_readlane(cur, page - base) : -1;
             }
-        }
-    };
-    auto fix = [&](Ptrs& a) {     // the table entries have arrived
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int e = __builtin_amdgcn_readfirstlane(a.phys[i]);
             a.phys[i] = (e >= 0 && e < p.map.n_blocks) ? e : -1;
         }
     };
-    auto step_of = [&](const Tile<D>& T, const Ptrs& a) {
-        const bool masked = a.phys[0] < 0 || a.phys[1] < 0 || a.tok[0] + 16 > min(seq_end, Q.lim_min) || a.tok[1] + 16 > min(seq_end, Q.lim_min);
-        if (masked) attend<D, NT, true>(Q, S, T, a, seq_end, lane);
-        else attend<D, NT, false>(Q, S, T, a, seq_end, lane);
+    const int end = min(seq_end, Q.lim_min);
+    auto compute = [&](const Tile<D>& T, const Ptrs& a) {
+        f32x4 x[2][NT];
+        u32x4 pb[NT];
+        const Params P = spread_params(T.par, stage, lane);
+        products<D, NT>(Q, T, x);
+        const bool masked = a.phys[0] < 0 || a.phys[1] < 0 || a.tok[0] + 16 > end || a.tok[1] + 16 > end;
+        const float top = masked ? scores<D, NT, true>(Q, S, P, a, seq_end, kg, x) : scores<D, NT, false>(Q, S, P, a, seq_end, kg, x);
+        float vs[2][4], vs_top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                vs[i][e] = lo16(P.v[i][e]) * S.inv_r;
+                if (masked && (a.phys[i] < 0 || a.tok[i] + 4 * kg + e >= seq_end)) vs[i][e] = 0.f;
+                vs_top = fmaxf(vs_top, vs[i][e]);
+            }
+        if (masked || S.open || __any(top > kLazy || vs_top > (float)(2 << kScaleTop))) move_references<D, NT>(S, x, vs, vs_top);
+        if (masked) weights<D, NT, true>(S, P, x, vs, pb);
+        else weights<D, NT, false>(S, P, x, vs, pb);
+        accumulate<D, NT>(S, T, pb);
     };
-    Tile<D> t0, t1;
-    Ptrs a0, a1;
-    locate(s, a0);
-    if (s + stride < s1) locate(s + stride, a1);
-    fix(a0);
-    load_tile<D>(p, R.kvh, a0, t0, lane);
+    Tile<D> T[DEPTH];
+    Ptrs a[DEPTH];
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+        locate(min(s + u * stride, last), a[u]);
+        load_tile<D, RW == 1>(p, R.kvh, a[u], T[u], lane);
+    }
+#pragma unroll 1
     while (true) {
-        Ptrs next;
-        const bool one = s + stride < s1, two = s + 2 * stride < s1;
-        if (two) locate(s + 2 * stride, next);
-        if (one) {
-            fix(a1);
-            load_tile<D>(p, R.kvh, a1, t1, lane);
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            compute(T[u], a[u]);
+            s += stride;
+            if (s >= s1) return;
+            locate(min(s + (DEPTH - 1) * stride, last), a[u]);
+            load_tile<D, RW == 1>(p, R.kvh, a[u], T[u], lane);
         }
-        step_of(t0, a0);
-        if (!one) break;
-        t0 = t1;
-        a0 = a1;
-        a1 = next;
-        s += stride;
     }
 }
 
 // One item, steps [s0, s1) of n_steps: the whole of it is written out, a part goes to the workspace and the last
 // workgroup to arrive merges.  part: where this workgroup's state goes; first / rest / stride / np: where all of them are.
-template <int D, int NT, bool ROWS, bool LIST>
+template <int D, int NT, int RW, bool LIST>
 __device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, int row0, int s0, int s1, bool whole,
                                          float* part, const float* first, const float* rest, long long stride, int np,
                                          unsigned* counter, const int2* list, int n_list, float* lds, int* flag, int wave, int lane) {
-    const int my_row0 = row0 + (ROWS ? wave * 16 * NT : 0);
+    const int my_row0 = row0 + wave % RW * 16 * NT;
     const int n_rows = min(p.rows_tile, R.n - row0);
     State<D, NT> S;
     clear_state(S);
     {
         Query<D, NT> Q;
         load_query<D, NT>(p, sq, R, my_row0, Q, lane);
-        walk<D, NT, ROWS, LIST>(p, sq, b, R, Q, S, s0, s1, list, n_list, wave, lane);
+        walk<D, NT, RW, LIST>(p, sq, b, R, Q, S, s0, s1, list, n_list, (uint32_t*)(flag + 4) + 64 * wave, wave, lane);
     }
     settle<D, NT>(S);
-    if (!ROWS) {
-        float* other = lds + 16 * NT * (D + 2);
+    // the waves that hold the same rows merge pairwise
+    float* const area[2] = {lds, lds + 16 * NT * (D + 2)};
+    if (RW < 4) {
         __syncthreads();                                  // the areas may still be read for the item before
-        if (wave & 1) state_to_lds<D, NT>(S, wave == 1 ? lds : other, lane);
+        const int odd = RW == 1 ? wave & 1 : wave >> 1, which = RW == 1 ? wave >> 1 : wave & 1;
+        if (odd) state_to_lds<D, NT>(S, area[which], lane);
         __syncthreads();
-        if (!(wave & 1)) merge_from_lds<D, NT>(S, wave == 0 ? lds : other, lane);
+        if (!odd) merge_from_lds<D, NT>(S, area[which], lane);
+    }
+    if (RW == 1) {
         __syncthreads();
         if (wave == 2) state_to_lds<D, NT>(S, lds, lane);
         __syncthreads();
         if (wave == 0) merge_from_lds<D, NT>(S, lds, lane);
     }
-    const bool mine = ROWS || wave == 0;
+    const bool mine = wave < RW;
     if (whole) {
         if (mine) write_out<D, NT>(p, R, my_row0, S, lane);
         return;
@@ -670,21 +754,21 @@ __device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq,
     __syncthreads();
 }
 
-template <int D, int NT, bool ROWS, bool LIST>
-__global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_attention_kernel(const Int4AttnParams p) {
+template <int D, int NT, int RW, bool LIST>
+__global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* lds = (float*)smem;
-    int* flag = (int*)(smem + Lds<D, NT, ROWS, LIST>::fixed - 16);
+    int* flag = (int*)(smem + Lds<D, NT, RW, LIST>::head);
     const int lane = lane_id(), wave = wave_id();
     const long long state = (long long)p.rows_tile * (D + 2);
 
     if constexpr (LIST) {
         const int item = blockIdx.x / p.workers, share = blockIdx.x - item * p.workers;
         const int b = item / p.list_rows, lr = item - b * p.list_rows;
-        const Seq sq = seq_of(p.map, b);
+        const Seq sq = uniform_seq(p.map, b);
         const bool per_head = p.list_rows == p.Hq;
         const Rows R{sq.first, per_head ? lr : lr * p.G, per_head ? 1 : p.G, per_head ? lr / p.G : lr, per_head ? 1 : p.G};
-        int2* list = (int2*)(smem + Lds<D, NT, ROWS, LIST>::fixed);
+        int2* list = (int2*)(smem + Lds<D, NT, RW, LIST>::fixed);
         // a list ends at its first entry outside the table (the sentinel among them): the shortest over the threads
         if (threadIdx.x == 0) *flag = p.P;
         __syncthreads();
@@ -698,11 +782,11 @@ __global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_at
         }
         if (end < p.P) atomicMin(flag, end);
         __syncthreads();
-        const int n_list = *flag;
+        const int n_list = uni(*flag);
         const int n_steps = (int)(((long long)n_list * p.map.block_size + kInt4StepTokens - 1) / kInt4StepTokens);
         const int s0 = (int)((long long)n_steps * share / p.workers), s1 = (int)((long long)n_steps * (share + 1) / p.workers);
         float* base = p.parts + (long long)item * p.workers * state;
-        run_item<D, NT, ROWS, LIST>(p, sq, b, R, 0, s0, s1, p.workers == 1, base + share * state, base, base + state, state, p.workers,
+        run_item<D, NT, RW, LIST>(p, sq, b, R, 0, s0, s1, p.workers == 1, base + share * state, base, base + state, state, p.workers,
                                     p.counters + item, list, n_list, lds, flag, wave, lane);
     } else {
         const int T = p.map.T, B = p.map.B;
@@ -726,7 +810,7 @@ __global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_at
             if (lanes_b) total += wave_sum(b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0);
             else total += head_steps_wave(p, seq_of(p.map, b0), lane);
         }
-        total *= p.Hkv;
+        total = uni(total) * p.Hkv;
         const long long piece = max((long long)p.min_steps, (total + p.workers - 1) / p.workers);
         long long g = (long long)w * piece;
         const long long g1 = min(total, g + piece);
@@ -754,9 +838,11 @@ __global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_at
                 off -= heads * p.Hkv;
             }
         }
-        b = __builtin_amdgcn_readfirstlane(b);
-        Seq sq = seq_of(p.map, b);
-        int h = __builtin_amdgcn_readfirstlane((int)(off / heads));
+        b = uni(b);
+        off = uni(off);
+        heads = uni(heads);
+        Seq sq = uniform_seq(p.map, b);
+        int h = uni((int)(off / heads));
         off -= h * heads;
         int rt = 0;
         if (!p.causal) {
@@ -777,16 +863,16 @@ __global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_at
                 off -= __shfl(incl, 63);
             }
         }
-        rt = __builtin_amdgcn_readfirstlane(rt);
-        int s0 = __builtin_amdgcn_readfirstlane((int)off);
+        rt = uni(rt);
+        int s0 = uni((int)off);
         while (true) {
-            const int n_steps = steps_of(p, sq, rt);
+            const int n_steps = uni(steps_of(p, sq, rt));
             const int s1 = (int)min((long long)n_steps, s0 + (g1 - g));
             const long long item0 = g - s0;
-            const int w0 = (int)(item0 / piece), w1 = (int)((item0 + n_steps - 1) / piece);
+            const int w0 = uni((int)(item0 / piece)), w1 = uni((int)((item0 + n_steps - 1) / piece));
             const Rows R{sq.first, h * p.G, p.G, h, sq.n * p.G};
             // slot 2 w + 1: the item begins in w's piece; slot 2 w: it began before
-            run_item<D, NT, ROWS, LIST>(p, sq, b, R, rt * p.rows_tile, s0, s1, w0 == w1, p.parts + (2ll * w + (s0 == 0)) * state,
+            run_item<D, NT, RW, LIST>(p, sq, b, R, rt * p.rows_tile, s0, s1, w0 == w1, p.parts + (2ll * w + (s0 == 0)) * state,
                                         p.parts + (2ll * w0 + 1) * state, p.parts + 2ll * (w0 + 1) * state, 2 * state, w1 - w0 + 1,
                                         p.counters + w0, nullptr, 0, lds, flag, wave, lane);
             g += s1 - s0;
@@ -796,17 +882,17 @@ __global__ __launch_bounds__(256, (NT * D <= 128 && !LIST) ? 2 : 1) void int4_at
                 rt = 0;
                 if (++h == p.Hkv) {
                     h = 0;
-                    do sq = seq_of(p.map, ++b); while (sq.n == 0);
+                    do sq = uniform_seq(p.map, ++b); while (sq.n == 0);
                 }
             }
         }
     }
 }
 
-template <int D, int NT, bool ROWS, bool LIST>
+template <int D, int NT, int RW, bool LIST>
 hipError_t launch_one(const Int4AttnParams& p, hipStream_t s, int* resident) {
-    auto kern = int4_attention_kernel<D, NT, ROWS, LIST>;
-    const size_t lds_bytes = (size_t)Lds<D, NT, ROWS, LIST>::fixed + (LIST ? (size_t)p.P * sizeof(int2) : 0);
+    auto kern = int4_attention_kernel<D, NT, RW, LIST>;
+    const size_t lds_bytes = (size_t)Lds<D, NT, RW, LIST>::fixed + (LIST ? (size_t)p.P * sizeof(int2) : 0);
     static int lds_limit[kMaxDevices];
     hipError_t e = ensure_lds_limit((const void*)kern, lds_limit, lds_bytes);
     if (e != hipSuccess) return e;
@@ -819,7 +905,7 @@ hipError_t launch_one(const Int4AttnParams& p, hipStream_t s, int* resident) {
         if (dev < 0 || dev >= kMaxDevices) return hipErrorInvalidDevice;
         std::lock_guard<std::mutex> lock(seen_mutex);
         if (seen[dev] == 0) {
-            e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, 256, (size_t)Lds<D, NT, ROWS, LIST>::fixed);
+            e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, 256, (size_t)Lds<D, NT, RW, LIST>::fixed);
             if (e != hipSuccess) return e;
             seen[dev] = (occ < 1 ? 1 : occ) * device_cu_count();
         }
@@ -833,17 +919,18 @@ hipError_t launch_one(const Int4AttnParams& p, hipStream_t s, int* resident) {
     return hipGetLastError();
 }
 
+template <int D, bool LIST>
+hipError_t dispatch(const Int4AttnParams& p, hipStream_t s, int* resident) {
+    constexpr int N = D <= 128 ? 2 : 1;      // row tiles of a wave (registers)
+    if (p.nt == 1 && p.row_waves == 1) return launch_one<D, 1, 1, LIST>(p, s, resident);
+    if constexpr (N == 2) if (p.nt == 2 && p.row_waves == 1) return launch_one<D, 2, 1, LIST>(p, s, resident);
+    if (p.nt == N && p.row_waves == 2) return launch_one<D, N, 2, LIST>(p, s, resident);
+    if (p.nt == N && p.row_waves == 4) return launch_one<D, N, 4, LIST>(p, s, resident);
+    return hipErrorInvalidConfiguration;
+}
 template <int D>
 hipError_t dispatch(const Int4AttnParams& p, hipStream_t s, int* resident) {
-    if (p.lists) {
-        if (p.nt == 1) return launch_one<D, 1, false, true>(p, s, resident);
-        if constexpr (D <= 128) if (p.nt == 4) return launch_one<D, 4, false, true>(p, s, resident);
-        return p.nt == 2 ? launch_one<D, 2, false, true>(p, s, resident) : hipErrorInvalidConfiguration;
-    }
-    if (p.by_rows) return p.nt == 2 ? launch_one<D, 2, true, false>(p, s, resident) : hipErrorInvalidConfiguration;
-    if (p.nt == 1) return launch_one<D, 1, false, false>(p, s, resident);
-    if constexpr (D <= 128) if (p.nt == 4) return launch_one<D, 4, false, false>(p, s, resident);
-    return p.nt == 2 ? launch_one<D, 2, false, false>(p, s, resident) : hipErrorInvalidConfiguration;
+    return p.lists ? dispatch<D, true>(p, s, resident) : dispatch<D, false>(p, s, resident);
 }
 hipError_t any_launch(const Int4AttnParams& p, hipStream_t s, int* resident) {
     switch (p.D) {

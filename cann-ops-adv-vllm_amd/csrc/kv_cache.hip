@@ -122,6 +122,7 @@ __device__ __forceinline__ void store8(void* base, long long off, int dtype, boo
 // The partner's value is read from the row again (a cache hit); all loads of a row come before its stores and one wave
 // holds the whole row, so the output may be the input itself.
 __device__ __forceinline__ void load_rotated(const AppendParams& p, const void* row, long long off, int c0, int cs_row, float* x) {
+#pragma clang fp contract(off)   // two rounded products and a rounded sum: the same value whichever of the paths below takes the row
     load8(row, off + c0, p.dtype, p.wide != 0, x);
     if (!p.cos_sin || c0 >= p.rot) return;
     const long long cs = (long long)cs_row * p.rot;
@@ -184,13 +185,14 @@ __device__ __forceinline__ uint32_t quantise8(const float* x, int lanes, int lan
         lo = fminf(lo, __shfl_xor(lo, step));
         hi = fmaxf(hi, __shfl_xor(hi, step));
     }
-    const _Float16 s = (_Float16)fminf((hi - lo) / 15.f, 65504.f);
+    const _Float16 s = (_Float16)fminf((hi - lo) * (1.f / 15.f), 65504.f);
     _Float16 z = (_Float16)fminf(fmaxf(lo, -65504.f), 65504.f);
-    const float zf = (float)z, inv = (float)s > 0.f ? 1.f / (float)s : 0.f;
+    // the division proper: 16-bit inputs meet exact halves often, and a reciprocal's rounding would decide those
+    const float zf = (float)z, sf = (float)s;
     uint32_t codes = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf((x[i] - zf) * inv), 0.f), 15.f);
+        const float c = sf > 0.f ? fminf(fmaxf(rintf((x[i] - zf) / sf), 0.f), 15.f) : 0.f;
         codes |= (uint32_t)(int)c << (4 * i);
     }
     uint16_t zb = __builtin_bit_cast(uint16_t, z), sb = __builtin_bit_cast(uint16_t, s);

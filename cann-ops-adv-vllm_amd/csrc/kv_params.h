@@ -91,8 +91,8 @@ struct Int4AttnParams {
     int list_rows, P;
     // plan
     int nt;                       // 16-row tiles a wave keeps
-    int by_rows;                  // 1: the four waves of a workgroup hold different rows, 0: different tokens
-    int rows_tile;                // rows of a work item (16 * nt, times 4 with by_rows)
+    int row_waves;                // 1, 2, 4: groups of rows among the four waves of a workgroup; the rest shares the tokens
+    int rows_tile;                // rows of a work item: 16 * nt * row_waves
     int workers;                  // workgroups (all tokens) / workgroups per list (n_split)
     int min_steps;                // fewest 32-token steps worth a workgroup of their own
     unsigned page_magic;          // ceil(2^32 / (block_size / 16)), 0 for a block size of 16

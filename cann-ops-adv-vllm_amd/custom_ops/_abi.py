@@ -194,3 +194,20 @@ def require_gpu(*tensors):
     for t in tensors:
         if isinstance(t, torch.Tensor) and t.numel() > 0 and not t.is_cuda:
             raise AclError("custom_ops operands must live on the GPU (there is no CPU implementation)")
+
+
+def _bind_native():
+    """The native binding of the KV-cache ops, handed the entry points of the library loaded above."""
+    try:
+        from . import _kv_binding as mod
+    except ImportError as e:
+        raise ImportError(f"custom_ops: the binding _kv_binding.so is missing or does not load ({e}). Build it with "
+                          "`make -C cann-ops-adv-vllm_amd/csrc` (or __graft_entry__.build())") from e
+    names = ["aclCreateTensor", "aclDestroyTensor", "aclCreateTensorList", "aclDestroyTensorList", "aclGetRecentErrMsg"]
+    for op in ("AppendKvCache", "GatherKvCache", "PagedAttentionInt4", "AssignBlockIds"):
+        names += [f"aclnn{op}GetWorkspaceSize", f"aclnn{op}"]
+    mod.bind(AclError, *(ctypes.cast(getattr(lib, n), c_void_p).value for n in names))
+    return mod
+
+
+native = _bind_native()

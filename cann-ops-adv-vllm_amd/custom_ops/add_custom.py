@@ -295,16 +295,8 @@ def assign_block_ids(key: torch.Tensor, block_table: torch.Tensor, seq_len: torc
     query row and the page gets the best cluster's id (ties: smallest id).  A page whose block_table entry lies outside
     the KV pool (the usual -1 of an unassigned slot) is skipped.  A decode loop calls this when a page
     fills up and advances first_new_page itself."""
-    _abi.require_gpu(key, block_table, seq_len, l1_cent, block_ids, first_new_page)
-    dev = key.device
-    kl = _abi.to_acl_list([key])
-    descs = [_abi.to_acl(t) for t in (block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset)]
-    ids_d = _abi.to_acl(block_ids)
-    try:
-        _abi.run(_abi.aclnnAssignBlockIdsGetWorkspaceSize, _abi.aclnnAssignBlockIds,
-                 [kl] + descs + [int(block_size), int(max_new_pages), ids_d], dev, "aclnnAssignBlockIds")
-    finally:
-        _destroy(descs + [ids_d], [kl])
+    _abi.native.assign(key, block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset, block_ids,
+                        int(block_size), int(max_new_pages))
     return block_ids
 
 

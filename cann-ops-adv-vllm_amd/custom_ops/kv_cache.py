@@ -20,7 +20,6 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _abi
-from .add_custom import _destroy
 
 
 class Int4Cache(NamedTuple):
@@ -38,14 +37,6 @@ def empty_int4_cache(num_blocks: int, num_key_value_heads: int, block_size: int,
     zeros = lambda shape, dt: torch.zeros(shape, dtype=dt, device=device)   # noqa: E731
     return Int4Cache(zeros((n, h, bs, d // 2), torch.uint8), zeros((n, h, bs // 4, d // 2, 4), torch.uint8),
                      zeros((n, h, bs, 2), torch.float16), zeros((n, h, bs, 2), torch.float16))
-
-
-def _one_device(what, *tensors):
-    """All operands on the GPU, and on the same one (they reach the kernel as bare addresses)."""
-    _abi.require_gpu(*tensors)
-    devs = {t.device for t in tensors if isinstance(t, torch.Tensor) and t.numel() > 0}
-    if len(devs) > 1:
-        raise _abi.AclError(f"{what}: operands on several devices {sorted(map(str, devs))}")
 
 
 def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -67,25 +58,9 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     same shapes (antiquant_scale / antiquant_offset as the attention ops take them, modes 0 and 2) or uint8: 4 bits, with
     key_params / value_params.  query_out may be query itself; where it is given, rows in no sequence are left as they are
     (a new tensor holds zeros there)."""
-    _one_device("append_kv_cache", key, value, key_cache, value_cache, block_table, seq_len, query, query_out, query_start, cos_sin,
-                positions, antiquant_scale, antiquant_offset, key_params, value_params)
-    own_out = query is not None and query_out is None
-    if query is None and query_out is not None:
-        raise _abi.AclError("append_kv_cache: query_out given without query")
-    if own_out:
-        query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    if key.dim() == 3 and key.shape[0] == 0:
-        return query_out                                     # no rows
-    descs = [_abi.to_acl(t) for t in (key, value, query, cos_sin, positions, block_table, seq_len, query_start, antiquant_scale,
-                                      antiquant_offset)]
-    outs = [_abi.to_acl(t) for t in (key_cache, value_cache, key_params, value_params, query_out)]
-    try:
-        _abi.run(_abi.aclnnAppendKvCacheGetWorkspaceSize, _abi.aclnnAppendKvCache,
-                 descs + [int(block_size), int(bool(interleaved)), int(antiquant_mode), int(own_out)] + outs, key.device,
-                 "aclnnAppendKvCache")
-    finally:
-        _destroy(descs + outs)
-    return query_out
+    return _abi.native.append(key, value, key_cache, value_cache, block_table, seq_len, query, query_out, query_start, cos_sin,
+                              positions, antiquant_scale, antiquant_offset, key_params, value_params, block_size,
+                              bool(interleaved), antiquant_mode)
 
 
 def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
@@ -99,8 +74,6 @@ def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_ta
     (K [T, Hkv, D], V).  num_tokens is T (needed with query_start, which lives on the GPU).  Tokens without a place in the
     cache read as zeros; rows in no sequence are zeros in new tensors and left as they are in key_out / value_out.
     out_dtype: float16 or bfloat16 (default: the cache's, the antiquant parameters' or float16)."""
-    _one_device("gather_kv_cache", key_cache, value_cache, block_table, seq_len, query_start, antiquant_scale, antiquant_offset,
-                key_params, value_params, key_out, value_out)
     if (key_out is None) != (value_out is None):
         raise _abi.AclError("gather_kv_cache: key_out and value_out come together")
     own_out = key_out is None
@@ -118,16 +91,9 @@ def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_ta
                 key_cache.dtype, key_cache.dtype)
         key_out = torch.empty((n, heads, d), dtype=out_dtype, device=key_cache.device)
         value_out = torch.empty_like(key_out)
-    if key_out.shape[0] == 0:
-        return key_out, value_out
-    descs = [_abi.to_acl(t) for t in (key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
-                                      antiquant_scale, antiquant_offset)]
-    outs = [_abi.to_acl(key_out), _abi.to_acl(value_out)]
-    try:
-        _abi.run(_abi.aclnnGatherKvCacheGetWorkspaceSize, _abi.aclnnGatherKvCache,
-                 descs + [int(block_size), int(antiquant_mode), int(own_out)] + outs, key_cache.device, "aclnnGatherKvCache")
-    finally:
-        _destroy(descs + outs)
+    if key_out.shape[0] > 0:
+        _abi.native.gather(key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start, antiquant_scale,
+                           antiquant_offset, key_out, value_out, block_size, antiquant_mode, own_out)
     return key_out, value_out
 
 
@@ -147,24 +113,11 @@ def paged_attention_int4(query: torch.Tensor, key_cache: torch.Tensor, value_cac
     block_position [B, Hq | Hkv, P] int32 (decode only): the logical pages each row attends, as cent_select returns them.
     softmax_lse: float32 [T, Hq], filled with the rows' log-sum-exp.  A row that sees no token is zero; rows in no sequence
     are zero in a new tensor and left as they are in `out`."""
-    _one_device("paged_attention_int4", query, key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
-                block_position, softmax_lse, out)
-    own_out = out is None
-    if own_out:
-        out = torch.empty(query.shape, dtype=out_dtype or query.dtype, device=query.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise _abi.AclError("paged_attention_int4: out and out_dtype disagree")
-    if query.dim() == 3 and query.shape[0] == 0:
-        return out
-    if max_query_len is None:
-        max_query_len = query.shape[0]
-    descs = [_abi.to_acl(t) for t in (query, key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
-                                      block_position)]
-    outs = [_abi.to_acl(out), _abi.to_acl(softmax_lse)]
-    try:
-        _abi.run(_abi.aclnnPagedAttentionInt4GetWorkspaceSize, _abi.aclnnPagedAttentionInt4,
-                 descs + [float(scale_value), int(num_key_value_heads), int(block_size), int(max_query_len), int(bool(causal)),
-                          int(own_out)] + outs, query.device, "aclnnPagedAttentionInt4")
-    finally:
-        _destroy(descs + outs)
-    return out
+    want = out.dtype if out is not None else query.dtype
+    if out_dtype is not None and out_dtype != want:
+        if out is not None or out_dtype != torch.float32:
+            raise _abi.AclError("paged_attention_int4: out_dtype must be query's dtype or float32, and out's where out is given")
+        want = out_dtype
+    return _abi.native.attention(query, key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start,
+                                 block_position, out, softmax_lse, scale_value, num_key_value_heads, block_size,
+                                 -1 if max_query_len is None else max_query_len, bool(causal), want == torch.float32)

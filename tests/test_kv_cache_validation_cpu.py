@@ -178,7 +178,7 @@ def test_attention_refusals(lib, over, word):
 def test_wide_groups_in_lists(lib):
     big = dict(q=t((5, 128, 256), F16), out=t((5, 128, 256), F16), **cache4(D=256))
     st, _, msg = attention(lib, lists=t((5, 2, 7), I32), **big)
-    assert st == INVALID and "group of 64" in msg
+    assert st == 0, msg
     assert attention(lib, lists=t((5, 128, 7), I32), **big)[0] == 0
 
 
