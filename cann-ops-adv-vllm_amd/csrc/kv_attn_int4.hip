@@ -48,9 +48,9 @@ constexpr float kNoMax = -3.0e38f;          // reference of a row that has seen 
 constexpr float kLazy = 8.f;                // log2 distance a reference may fall behind the true maximum
 constexpr int kScaleTop = 6;                // V scales are brought below 2^6 (and may grow to 2^7 before the next slow path)
 
-// A step: for each half of 16 tokens the physical page (< 0: nothing there), the row in it and the token's place in the
-// sequence.
-struct Ptrs { int phys[2], row[2], tok[2]; };
+// A step: for each half of 16 tokens the row of the cache where it begins, the first token's place in the sequence, and
+// whether the page is there.
+struct Ptrs { long long row[2]; int tok[2]; bool ok[2]; };
 
 template <int W> struct Words { uint32_t w[W]; };
 // STREAM: bytes that nobody reads again soon (decode): 268 -> 250 us for 1.4 GB against ordinary loads
@@ -276,33 +276,28 @@ struct Tile {
     Words<D / 32> k[2], v[2];
     uint32_t par;
 };
-// First row of a half step in the codes and parameters: row index over the whole cache.
-__device__ __forceinline__ long long row_at(const Int4AttnParams& p, int kvh, const Ptrs& a, int i) {
-    return ((long long)max(a.phys[i], 0) * p.Hkv + kvh) * p.map.block_size + a.row[i];
-}
+// par: the lane's place in the parameters of a page's first row (K for lanes 0 .. 31, V behind)
 template <int D, bool STREAM>
-__device__ __forceinline__ void load_tile(const Int4AttnParams& p, int kvh, const Ptrs& a, Tile<D>& t, int lane) {
-    const long long r0 = row_at(p, kvh, a, 0), r1 = row_at(p, kvh, a, 1);
-    const long long rp = (lane & 16) ? r1 : r0;
-    t.par = (lane < 32 ? p.k_params : p.v_params)[rp + (lane & 15)];
+__device__ __forceinline__ void load_tile(const Int4AttnParams& p, const uint32_t* par, const Ptrs& a, Tile<D>& t, int lane) {
+    t.par = par[p.paired ? a.row[0] : ((lane & 16) ? a.row[1] - 16 : a.row[0])];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const long long row = i ? r1 : r0;
-        t.k[i] = load_words<D / 32, STREAM>(p.kcache + row * (D / 2) + (unsigned)((lane & 15) * (D / 2) + (lane >> 4) * (D / 8)));
-    }
+    for (int i = 0; i < 2; ++i)
+        t.k[i] = load_words<D / 32, STREAM>(p.kcache + a.row[i] * (D / 2) + (unsigned)((lane & 15) * (D / 2) + (lane >> 4) * (D / 8)));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const long long row = i ? r1 : r0;
-        t.v[i] = load_words<D / 32, STREAM>(p.vcache + row * (D / 2) + (unsigned)((lane >> 4) * (2 * D) + (lane & 15) * (D / 8)));
-    }
+    for (int i = 0; i < 2; ++i)
+        t.v[i] = load_words<D / 32, STREAM>(p.vcache + a.row[i] * (D / 2) + (unsigned)((lane >> 4) * (2 * D) + (lane & 15) * (D / 8)));
 }
 struct Params { u32x4 k[2], v[2]; };     // of the lane's four tokens in each half
 __device__ __forceinline__ Params spread_params(uint32_t par, uint32_t* stage, int lane) {
-    wave_lds_sync();                     // (the reads of the step before are done)
+    // LDS serves a wave in order: neither the write after the reads of the step before nor these reads after the write
+    // need a wait, only the compiler has to keep the order (the first product runs while they are on their way)
+    asm volatile("" ::: "memory");
     stage[lane] = par;
-    wave_lds_sync();
+    asm volatile("" ::: "memory");
     const u32x4* at = (const u32x4*)(stage + (lane >> 4) * 4);
-    return Params{{at[0], at[4]}, {at[8], at[12]}};
+    const Params r{{at[0], at[4]}, {at[8], at[12]}};
+    asm volatile("" ::: "memory");
+    return r;
 }
 
 // A step in three parts.  MASKED: some token of the step is hidden from some row (the end of the sequence, the causal
@@ -335,10 +330,24 @@ __device__ __forceinline__ float scores(const Query<D, NT>& Q, const State<D, NT
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float x = fmaf(s[i][t][e], ks, fmaf(kz, Q.sum[t], -S.m[t]));
-                if (MASKED && (a.phys[i] < 0 || tok >= min(seq_end, Q.lim[t]))) x = -__builtin_inff();
+                if (MASKED && (!a.ok[i] || tok >= min(seq_end, Q.lim[t]))) x = -__builtin_inff();
                 s[i][t][e] = x;
                 top = fmaxf(top, x);
             }
+        }
+    return top;
+}
+// V scales of the lane's tokens over the scale reference, largest of them
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ float value_scales(const State<D, NT>& S, const Params& P, const Ptrs& a, int seq_end, int kg, float (&vs)[2][4]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            vs[i][e] = lo16(P.v[i][e]) * S.inv_r;
+            if (MASKED && (!a.ok[i] || a.tok[i] + 4 * kg + e >= seq_end)) vs[i][e] = 0.f;
+            top = fmaxf(top, vs[i][e]);
         }
     return top;
 }
@@ -426,8 +435,8 @@ __device__ __forceinline__ void accumulate(State<D, NT>& S, const Tile<D>& T, co
 }
 
 // ---- finished states ------------------------------------------------------------------------------------------------
-// Per row: D un-normalised outputs, the reference m (log2) and the sum l; a row without tokens has m = kNoMax, l = 0.
-// In registers of a wave: State with o in real units and m, l complete in every lane of the row.
+// Per row: D un-normalised outputs, the reference m (log2) and the sum l, complete in every lane of the row; a row without
+// tokens has m = kNoMax, l = 0.
 template <int D, int NT>
 __device__ __forceinline__ void settle(State<D, NT>& S) {
     const float even = 16777216.f / S.inv_r, odd = even * 0.0625f, mid = 7.5f / S.inv_r;
@@ -512,46 +521,52 @@ __device__ __forceinline__ Pair ld_pair(const float* ptr) {
     v.u = ld_agent((const unsigned long long*)ptr);
     return v;
 }
+// A partial state in the workspace, tile by tile of 16 rows as the lanes hold it, so that every access is 512 contiguous
+// bytes: [tile][d][pair of o's elements][lane] pairs of outputs, then [tile][lane] (m, l).
+template <int D> constexpr int part_tile_floats() { return (D / 16 * 2 + 1) * 128; }
 template <int D, int NT>
-__device__ __forceinline__ void state_to_parts(const State<D, NT>& S, float* st, int row0, int n_rows, int lane) {
-    const int n = lane & 15, kg = lane >> 4;
+__device__ __forceinline__ void state_to_part(const State<D, NT>& S, float* part, int tile0, int n_rows, int lane) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 16 * t + n;
-        if (r >= n_rows) continue;
-        float* row = st + (long long)r * (D + 2);
+        if ((tile0 + t) * 16 >= n_rows) break;
+        float* at = part + (long long)(tile0 + t) * part_tile_floats<D>() + 2 * lane;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < D / 16; d += 2) st_pair(row + kg * (D / 4) + i * (D / 16) + d, S.o[t][d][i], S.o[t][d + 1][i]);
-        if (kg == 0) st_pair(row + D, S.m[t], S.l[t]);
+        for (int d = 0; d < D / 16; ++d) {
+            st_pair(at + (2 * d) * 128, S.o[t][d][0], S.o[t][d][1]);
+            st_pair(at + (2 * d + 1) * 128, S.o[t][d][2], S.o[t][d][3]);
+        }
+        st_pair(at + (D / 16 * 2) * 128, S.m[t], S.l[t]);
     }
 }
 
 // The last workgroup to arrive at a split item merges its np partial states, which lie `stride` floats apart except for
-// the first.  D / 4 threads share a row, four channels each; where rows are fewer than the 1024 / D groups of threads,
-// several groups take every sub-th part of a row and join through LDS.
-template <int D>
+// the first.  The waves share the tiles, or the channels of a tile where tiles are fewer; the loads of BATCH states are
+// under way at once (they come past the caches, about 2 us each).
+template <int D, int TILES>
 __device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows& R, int row0, int n_rows, const float* first,
-                                            const float* rest, long long stride, int np, float* lds) {
-    constexpr int TPR = D / 4, SLOTS = 256 / TPR, BATCH = 8;
-    const int slot = threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
-    int sub = 1;
-    while (sub * 2 * n_rows <= SLOTS && sub * 2 <= np) sub *= 2;
-    const int per_pass = SLOTS / sub, sid = slot % sub;
-    for (int base = 0; base < n_rows; base += per_pass) {
-        const int r = base + slot / sub;
-        const bool live = r < n_rows;
-        float m = kNoMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int p0 = sid; p0 < np && live; p0 += BATCH * sub) {
-            Pair ml[BATCH], a[BATCH], b[BATCH];
+                                            const float* rest, long long stride, int np, int wave, int lane) {
+    constexpr int WANT = TILES >= 4 ? 1 : 4 / TILES, SHARE = WANT < D / 32 ? WANT : D / 32;   // waves of a tile
+    constexpr int DW = D / 16 / SHARE;                         // d's of a wave
+    constexpr int BATCH = DW <= 2 ? 8 : (DW <= 8 ? 4 : 2);
+    const int n = lane & 15, kg = lane >> 4, d0 = wave % SHARE * DW;
+    for (int tile = wave / SHARE; tile * 16 < n_rows; tile += 4 / SHARE) {
+        const long long off = (long long)tile * part_tile_floats<D>() + 2 * lane;
+        float m = kNoMax, l = 0.f;
+        f32x4 o[DW];
+#pragma unroll
+        for (int d = 0; d < DW; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < np; p0 += BATCH) {
+            Pair ml[BATCH], a[BATCH][DW], b[BATCH][DW];
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
-                const int j = min(p0 + u * sub, np - 1);
-                const float* row = (j == 0 ? first : rest + (long long)(j - 1) * stride) + (long long)r * (D + 2);
-                ml[u] = ld_pair(row + D);
-                a[u] = ld_pair(row + c);
-                b[u] = ld_pair(row + c + 2);
+                const int j = min(p0 + u, np - 1);
+                const float* at = (j == 0 ? first : rest + (long long)(j - 1) * stride) + off;
+                ml[u] = ld_pair(at + (D / 16 * 2) * 128);
+#pragma unroll
+                for (int d = 0; d < DW; ++d) {
+                    a[u][d] = ld_pair(at + (2 * (d0 + d)) * 128);
+                    b[u][d] = ld_pair(at + (2 * (d0 + d) + 1) * 128);
+                }
             }
             float top = m;
 #pragma unroll
@@ -560,42 +575,28 @@ __device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows&
             m = top;
             l *= keep;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] *= keep;
+            for (int d = 0; d < DW; ++d) o[d] *= keep;
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const float f = p0 + u * sub < np ? fast_exp2(ml[u].f[0] - top) : 0.f;
-                if (p0 + u * sub < np) {
+            for (int u = 0; u < BATCH; ++u)
+                if (p0 + u < np) {
+                    const float f = fast_exp2(ml[u].f[0] - top);
                     l += ml[u].f[1] * f;
-                    o[0] += a[u].f[0] * f; o[1] += a[u].f[1] * f; o[2] += b[u].f[0] * f; o[3] += b[u].f[1] * f;
-                }
-            }
-        }
-        if (sub > 1) {
-            float* st = lds + slot * (D + 2);
-            __syncthreads();
-            if (sid != 0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) st[c + e] = o[e];
-                if (c == 0) { st[D] = m; st[D + 1] = l; }
-            }
-            __syncthreads();
-            if (sid == 0)
-                for (int u = 1; u < sub; ++u) {
-                    const float* ot = lds + (slot + u) * (D + 2);
-                    const float mo = ot[D], lo = ot[D + 1], top = fmaxf(m, mo), f = fast_exp2(m - top), g = fast_exp2(mo - top);
-                    m = top;
-                    l = l * f + lo * g;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + ot[c + e] * g;
+                    for (int d = 0; d < DW; ++d)
+                        o[d] += f32x4{a[u][d].f[0] * f, a[u][d].f[1] * f, b[u][d].f[0] * f, b[u][d].f[1] * f};
                 }
         }
-        if (live && sid == 0) {
+        const int r = tile * 16 + n;
+        if (r < n_rows) {
             const int rr = row0 + r, i0 = rr / R.G, head = R.head0 + rr - i0 * R.G;
             const long long row = (long long)(R.first + i0) * p.Hq + head;
             const float f = out_factor(l);
-            put_out(p, row * D + c, o[0] * f, o[1] * f);
-            put_out(p, row * D + c + 2, o[2] * f, o[3] * f);
-            if (p.lse && c == 0) p.lse[row] = lse_of(m, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < DW; d += 2)
+                    put_out(p, row * D + kg * (D / 4) + i * (D / 16) + d0 + d, o[d][i] * f, o[d + 1][i] * f);
+            if (p.lse && kg == 0 && d0 == 0) p.lse[row] = lse_of(m, l);
         }
     }
 }
@@ -604,8 +605,7 @@ __device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows&
 template <int D, int NT, int RW, bool LIST>
 struct Lds {
     static constexpr int merge = RW == 4 ? 0 : 2 * 16 * NT * (D + 2) * 4;   // two states
-    static constexpr int join = (1024 / D) * (D + 2) * 4;
-    static constexpr int head = (merge > join ? merge : join);
+    static constexpr int head = merge;
     static constexpr int fixed = head + 16 + 1024;   // the flag, 256 bytes of parameters per wave
 };
 // Steps whose data is under way, and waves per SIMD that the registers of a variant are cut for.
@@ -639,46 +639,53 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
         cur = entries(base);
         nxt = entries(base + 64);
     }
-    auto locate = [&](int step, Ptrs& a) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const unsigned u = 2u * (unsigned)step + i;
-            const int page = page_of(u);
-            a.row[i] = (int)(16u * u) - page * bs;
-            int e;
-            if (LIST) {
-                const int2 le = page < n_list ? list[page] : make_int2(0, -1);
-                a.tok[i] = uni(le.x) * bs + a.row[i];
-                e = uni(le.y);
-            } else {
-                a.tok[i] = (int)(16u * u);
-                while (page - base >= 64) {
-                    cur = nxt;
-                    base += 64;
-                    nxt = entries(base + 64);
-                }
-                e = a.tok[i] < seq_end ? __builtin_amdgcn_readlane(cur, page - base) : -1;
+    const int page_rows = p.Hkv * bs, first_row = R.kvh * bs;
+    auto place = [&](int step, int i, Ptrs& a) {
+        const unsigned u = 2u * (unsigned)step + i;
+        const int page = page_of(u), in_page = (int)(16u * u) - page * bs;
+        int e;
+        if (LIST) {
+            const int2 le = page < n_list ? list[page] : make_int2(0, -1);
+            a.tok[i] = uni(le.x) * bs + in_page;
+            e = uni(le.y);
+        } else {
+            a.tok[i] = (int)(16u * u);
+            while (page - base >= 64) {
+                cur = nxt;
+                base += 64;
+                nxt = entries(base + 64);
             }
-            a.phys[i] = (e >= 0 && e < p.map.n_blocks) ? e : -1;
+            e = a.tok[i] < seq_end ? __builtin_amdgcn_readlane(cur, page - base) : -1;
+        }
+        a.ok[i] = (unsigned)e < (unsigned)p.map.n_blocks;
+        a.row[i] = (long long)(a.ok[i] ? e : 0) * page_rows + (first_row + in_page);
+    };
+    auto locate = [&](int step, Ptrs& a) {
+        place(step, 0, a);
+        if (p.paired) {                     // both halves in one page
+            a.row[1] = a.row[0] + 16;
+            a.tok[1] = a.tok[0] + 16;
+            a.ok[1] = a.ok[0];
+        } else {
+            place(step, 1, a);
         }
     };
+    const uint32_t* par = (lane < 32 ? p.k_params : p.v_params) + (lane & 31);
     const int end = min(seq_end, Q.lim_min);
     auto compute = [&](const Tile<D>& T, const Ptrs& a) {
         f32x4 x[2][NT];
         u32x4 pb[NT];
         const Params P = spread_params(T.par, stage, lane);
         products<D, NT>(Q, T, x);
-        const bool masked = a.phys[0] < 0 || a.phys[1] < 0 || a.tok[0] + 16 > end || a.tok[1] + 16 > end;
-        const float top = masked ? scores<D, NT, true>(Q, S, P, a, seq_end, kg, x) : scores<D, NT, false>(Q, S, P, a, seq_end, kg, x);
-        float vs[2][4], vs_top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                vs[i][e] = lo16(P.v[i][e]) * S.inv_r;
-                if (masked && (a.phys[i] < 0 || a.tok[i] + 4 * kg + e >= seq_end)) vs[i][e] = 0.f;
-                vs_top = fmaxf(vs_top, vs[i][e]);
-            }
+        const bool masked = !a.ok[0] || !a.ok[1] || max(a.tok[0], a.tok[1]) + 16 > end;
+        float vs[2][4], top, vs_top;
+        if (masked) {
+            top = scores<D, NT, true>(Q, S, P, a, seq_end, kg, x);
+            vs_top = value_scales<D, NT, true>(S, P, a, seq_end, kg, vs);
+        } else {
+            top = scores<D, NT, false>(Q, S, P, a, seq_end, kg, x);
+            vs_top = value_scales<D, NT, false>(S, P, a, seq_end, kg, vs);
+        }
         if (masked || S.open || __any(top > kLazy || vs_top > (float)(2 << kScaleTop))) move_references<D, NT>(S, x, vs, vs_top);
         if (masked) weights<D, NT, true>(S, P, x, vs, pb);
         else weights<D, NT, false>(S, P, x, vs, pb);
@@ -689,7 +696,7 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
         locate(min(s + u * stride, last), a[u]);
-        load_tile<D, RW == 1>(p, R.kvh, a[u], T[u], lane);
+        load_tile<D, RW == 1>(p, par, a[u], T[u], lane);
     }
 #pragma unroll 1
     while (true) {
@@ -699,7 +706,7 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
             s += stride;
             if (s >= s1) return;
             locate(min(s + (DEPTH - 1) * stride, last), a[u]);
-            load_tile<D, RW == 1>(p, R.kvh, a[u], T[u], lane);
+            load_tile<D, RW == 1>(p, par, a[u], T[u], lane);
         }
     }
 }
@@ -740,7 +747,7 @@ __device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq,
         if (mine) write_out<D, NT>(p, R, my_row0, S, lane);
         return;
     }
-    if (mine) state_to_parts<D, NT>(S, part, my_row0 - row0, n_rows, lane);
+    if (mine) state_to_part<D, NT>(S, part, wave % RW * NT, n_rows, lane);
     wait_stores();
     __syncthreads();
     if (threadIdx.x == 0)
@@ -749,7 +756,7 @@ __device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq,
     const int last = *flag;
     if (last) {
         if (threadIdx.x == 0) st_agent(counter, 0u);      // left as found: the next launch on this workspace counts again
-        merge_parts<D>(p, R, row0, n_rows, first, rest, stride, np, lds);
+        merge_parts<D, NT * RW>(p, R, row0, n_rows, first, rest, stride, np, wave, lane);
     }
     __syncthreads();
 }
@@ -760,7 +767,7 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
     float* lds = (float*)smem;
     int* flag = (int*)(smem + Lds<D, NT, RW, LIST>::head);
     const int lane = lane_id(), wave = wave_id();
-    const long long state = (long long)p.rows_tile * (D + 2);
+    constexpr long long state = (long long)NT * RW * part_tile_floats<D>();
 
     if constexpr (LIST) {
         const int item = blockIdx.x / p.workers, share = blockIdx.x - item * p.workers;
@@ -804,11 +811,15 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
         const int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
         if (w >= p.workers) return;
         // the line of steps: its length, and where this workgroup's piece begins
-        const bool lanes_b = B >= 16;     // a lane per sequence, or the wave over the row tiles of each
-        long long total = 0;
+        const bool lanes_b = B >= 16 || p.most_tiles <= 4;     // a lane per sequence, or the wave over the row tiles of each
+        long long total = 0, mine = 0;
         for (int b0 = 0; b0 < B; b0 += lanes_b ? 64 : 1) {
-            if (lanes_b) total += wave_sum(b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0);
-            else total += head_steps_wave(p, seq_of(p.map, b0), lane);
+            if (lanes_b) {
+                mine = b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
+                total += wave_sum(mine);
+            } else {
+                total += head_steps_wave(p, seq_of(p.map, b0), lane);
+            }
         }
         total = uni(total) * p.Hkv;
         const long long piece = max((long long)p.min_steps, (total + p.workers - 1) / p.workers);
@@ -819,13 +830,13 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
         long long off = g, heads = 0;
         if (lanes_b) {
             for (int b0 = 0; b0 < B; b0 += 64) {
-                const long long mine = b0 + lane < B ? p.Hkv * head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
-                const long long incl = wave_scan(mine, lane);
+                if (B > 64) mine = b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
+                const long long incl = wave_scan(mine, lane) * p.Hkv;
                 const unsigned long long past = __ballot(incl > off);
                 if (past) {
                     const int at = __ffsll(past) - 1;
-                    off -= __shfl(incl - mine, at);
-                    heads = __shfl(mine, at) / p.Hkv;
+                    heads = __shfl(mine, at);
+                    off -= __shfl(incl, at) - heads * p.Hkv;
                     b = b0 + at;
                     break;
                 }
@@ -851,12 +862,12 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
         } else {
             const int nt = row_tiles(p, sq);
             for (int r0 = 0; r0 < nt; r0 += 64) {
-                const long long mine = r0 + lane < nt ? steps_of(p, sq, r0 + lane) : 0;
-                const long long incl = wave_scan(mine, lane);
+                const long long tile = r0 + lane < nt ? steps_of(p, sq, r0 + lane) : 0;
+                const long long incl = wave_scan(tile, lane);
                 const unsigned long long past = __ballot(incl > off);
                 if (past) {
                     const int at = __ffsll(past) - 1;
-                    off -= __shfl(incl - mine, at);
+                    off -= __shfl(incl - tile, at);
                     rt = r0 + at;
                     break;
                 }
@@ -945,6 +956,7 @@ hipError_t any_launch(const Int4AttnParams& p, hipStream_t s, int* resident) {
 }  // namespace
 
 hipError_t launch_int4_attention(const Int4AttnParams& p, hipStream_t s) { return any_launch(p, s, nullptr); }
+long long int4_attention_part_bytes(const Int4AttnParams& p) { return (long long)(p.rows_tile / 16) * (p.D / 16 * 2 + 1) * 128 * 4; }
 int int4_attention_resident(const Int4AttnParams& p) {
     int n = 0;
     if (device_cu_count() <= 0 || any_launch(p, nullptr, &n) != hipSuccess) { (void)hipGetLastError(); return 0; }

@@ -93,8 +93,10 @@ struct Int4AttnParams {
     int nt;                       // 16-row tiles a wave keeps
     int row_waves;                // 1, 2, 4: groups of rows among the four waves of a workgroup; the rest shares the tokens
     int rows_tile;                // rows of a work item: 16 * nt * row_waves
+    int most_tiles;               // work items of one (sequence, kv head), at most
     int workers;                  // workgroups (all tokens) / workgroups per list (n_split)
     int min_steps;                // fewest 32-token steps worth a workgroup of their own
+    int paired;                   // 32 tokens never cross a page (block_size a multiple of 32)
     unsigned page_magic;          // ceil(2^32 / (block_size / 16)), 0 for a block size of 16
     unsigned* counters;           // arrivals per split item, zeroed before and left zeroed
     float* parts;                 // partial states
@@ -105,7 +107,8 @@ hipError_t launch_gather(const GatherParams& p, hipStream_t s);
 hipError_t launch_int4_attention(const Int4AttnParams& p, hipStream_t s);
 // Workgroups of the planned kernel that the current device holds at once (0: no device).
 int int4_attention_resident(const Int4AttnParams& p);
-// Workgroups that share the work of a call: one partial state slot pair each (lists: workers per list, one slot each).
+// Bytes of one partial state (two per workgroup; with page lists one per workgroup).
+long long int4_attention_part_bytes(const Int4AttnParams& p);
 constexpr int kInt4StepTokens = 32;
 constexpr int kInt4MaxList = 4096;     // entries of a page list (8 bytes of LDS each)
 
