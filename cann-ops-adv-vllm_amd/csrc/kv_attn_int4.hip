@@ -41,7 +41,6 @@ namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;          // reference of a row that has seen no token
@@ -53,22 +52,14 @@ constexpr int kScaleTop = 6;                // V scales are brought below 2^6 (a
 struct Ptrs { long long row[2]; int tok[2]; bool ok[2]; };
 
 template <int W> struct Words { uint32_t w[W]; };
-// STREAM: bytes that nobody reads again soon (decode): 268 -> 250 us for 1.4 GB against ordinary loads
-template <int W, bool STREAM>
+template <int W>
 __device__ __forceinline__ Words<W> load_words(const uint8_t* p) {
-    auto ld = [](auto* a) {
-        if constexpr (STREAM) return __builtin_nontemporal_load(a);
-        else return *a;
-    };
     Words<W> r;
-    if constexpr (W == 1) r.w[0] = ld((const uint32_t*)p);
-    else if constexpr (W == 2) { const u32x2 v = ld((const u32x2*)p); r.w[0] = v[0]; r.w[1] = v[1]; }
+    if constexpr (W == 1) r.w[0] = *(const uint32_t*)p;
+    else if constexpr (W == 2) { const uint2 v = *(const uint2*)p; r.w[0] = v.x; r.w[1] = v.y; }
     else {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const u32x4 v = ld((const u32x4*)(p + 16 * i));
-            r.w[4 * i] = v[0]; r.w[4 * i + 1] = v[1]; r.w[4 * i + 2] = v[2]; r.w[4 * i + 3] = v[3];
-        }
+        const uint4 v = *(const uint4*)p;
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
     }
     return r;
 }
@@ -123,10 +114,6 @@ __device__ __forceinline__ int steps_of(const Int4AttnParams& p, const Seq& s, i
 }
 __device__ __forceinline__ int row_tiles(const Int4AttnParams& p, const Seq& s) { return (s.n * p.G + p.rows_tile - 1) / p.rows_tile; }
 
-__device__ __forceinline__ long long wave_sum(long long x) {
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
-}
 __device__ __forceinline__ long long wave_scan(long long x, int lane) {   // inclusive
     for (int d = 1; d < 64; d <<= 1) {
         const long long up = __shfl_up(x, d);
@@ -134,6 +121,25 @@ __device__ __forceinline__ long long wave_scan(long long x, int lane) {   // inc
     }
     return x;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int x, int) {
+    x = dpp_add<0x111, 0xf>(x);      // row_shr 1, 2, 4, 8: inclusive within 16 lanes
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);      // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+    return dpp_add<0x143, 0xc>(x);
+}
+__device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ long long lane_of(long long x, int lane) {
+    return (long long)(((unsigned long long)(unsigned)lane_of((int)((unsigned long long)x >> 32), lane) << 32) | (unsigned)lane_of((int)x, lane));
+}
+// non-negative; the 64-bit division is a long routine and hardly ever needed
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (((unsigned long long)a | (unsigned long long)b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // steps of one kv head of a sequence (all its row tiles), computed by one lane / by the wave
 __device__ __forceinline__ long long head_steps_lane(const Int4AttnParams& p, const Seq& s) {
     const int nt = row_tiles(p, s);
@@ -143,12 +149,87 @@ __device__ __forceinline__ long long head_steps_lane(const Int4AttnParams& p, co
     for (int rt = 0; rt < nt; ++rt) t += steps_of(p, s, rt);
     return t;
 }
-__device__ __forceinline__ long long head_steps_wave(const Int4AttnParams& p, const Seq& s, int lane) {
+template <typename I>
+__device__ __forceinline__ I head_steps_wave(const Int4AttnParams& p, const Seq& s, int lane) {
     const int nt = row_tiles(p, s);
-    if (!p.causal) return nt > 0 ? (long long)nt * steps_of(p, s, 0) : 0;
-    long long t = 0;
+    if (!p.causal) return nt > 0 ? (I)nt * steps_of(p, s, 0) : 0;
+    I t = 0;
     for (int rt = lane; rt < nt; rt += 64) t += steps_of(p, s, rt);
-    return wave_sum(t);
+    return lane_of(wave_scan(t, lane), 63);
+}
+
+// A workgroup's piece [g, g1) of the line of all steps, and where it begins: step s0 of row tile rt of kv head h of sequence b.
+struct Piece { long long g, g1, size; int b, h, rt, s0; };
+// I: 32 bits where the line is known to be short enough (64-bit scans and divisions cost microseconds here)
+template <typename I>
+__device__ __forceinline__ bool find_piece(const Int4AttnParams& p, int w, int lane, Piece& out) {
+    const int B = p.map.B;
+    const bool lanes_b = B >= 16 || p.most_tiles <= 4;     // a lane per sequence, or the wave over the row tiles of each
+    I total = 0, mine = 0, incl = 0;
+    for (int b0 = 0; b0 < B; b0 += lanes_b ? 64 : 1) {
+        if (lanes_b) {
+            mine = b0 + lane < B ? (I)head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
+            incl = wave_scan(mine, lane);
+            total += lane_of(incl, 63);
+        } else {
+            total += head_steps_wave<I>(p, uniform_seq(p.map, b0), lane);
+        }
+    }
+    total *= p.Hkv;
+    out.size = max((long long)p.min_steps, quotient((long long)total + p.workers - 1, p.workers));
+    out.g = w * out.size;
+    if (out.g >= total) return false;
+    out.g1 = min((long long)total, out.g + out.size);
+    I off = (I)out.g, heads = 0;
+    int b = 0;
+    if (lanes_b) {
+        for (int b0 = 0; b0 < B; b0 += 64) {
+            if (B > 64) {
+                mine = b0 + lane < B ? (I)head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
+                incl = wave_scan(mine, lane);
+            }
+            const unsigned long long past = __ballot(incl * p.Hkv > off);
+            if (past) {
+                const int at = __ffsll(past) - 1;
+                heads = lane_of(mine, at);
+                off -= (lane_of(incl, at) - heads) * p.Hkv;
+                b = b0 + at;
+                break;
+            }
+            off -= lane_of(incl, 63) * p.Hkv;
+        }
+    } else {
+        for (;; ++b) {
+            heads = head_steps_wave<I>(p, uniform_seq(p.map, b), lane);
+            if (off < heads * p.Hkv) break;
+            off -= heads * p.Hkv;
+        }
+    }
+    out.b = uni(b);
+    const Seq sq = uniform_seq(p.map, out.b);
+    out.h = uni((int)quotient(off, heads));
+    off -= out.h * heads;
+    int rt = 0;
+    if (!p.causal) {
+        const int n = steps_of(p, sq, 0);
+        rt = (int)quotient(off, n);
+        off -= (I)rt * n;
+    } else if (row_tiles(p, sq) > 1) {
+        for (int r0 = 0;; r0 += 64) {
+            const I tile = r0 + lane < row_tiles(p, sq) ? steps_of(p, sq, r0 + lane) : 0, upto = wave_scan(tile, lane);
+            const unsigned long long past = __ballot(upto > off);
+            if (past) {
+                const int at = __ffsll(past) - 1;
+                off -= lane_of(upto, at) - lane_of(tile, at);
+                rt = r0 + at;
+                break;
+            }
+            off -= lane_of(upto, 63);
+        }
+    }
+    out.rt = uni(rt);
+    out.s0 = uni((int)off);
+    return true;
 }
 
 // ---- the state of a wave -------------------------------------------------------------------------------------------
@@ -187,130 +268,177 @@ struct Query {
 // What the rows of a work item are: row r is token first + r / G of the sequence, q head head0 + r % G.
 struct Rows { int first, head0, G, kvh, n; };
 
-// q rows [row0, row0 + 16 NT) of an item -> operand B.  The rows of a wave are brought to a common power of two with the
-// largest element in [2^10, 2^11): float16 then holds every element down to 2^-25 of it exactly (bfloat16 rows outside
-// float16's range included), and the even slots, 16 times larger, stay below 2^15.
 template <int D, int NT>
-__device__ __forceinline__ void load_query(const Int4AttnParams& p, const Seq& s, const Rows& R, int row0, Query<D, NT>& Q, int lane) {
-    constexpr int W = D / 32;                 // 16-byte pieces (8 channels) of a lane
-    const int n = lane & 15, kg = lane >> 4;
-    const bool bf = p.q_dtype == kBF16;
-    // eight channels of the lane's row of tile t
-    auto piece = [&](int t, int j, float (&x)[8]) {
-        const int r = row0 + 16 * t + n;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (r < R.n) {
-            const int i = r / R.G;
-            const uint16_t* src = (const uint16_t*)p.q + (long long)(R.first + i) * p.q_tok + (long long)(R.head0 + r - i * R.G) * p.q_head +
-                                  kg * 8 * W + 8 * j;
-            if (p.q_wide) {
-                const uint4 v = *(const uint4*)src;
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-            } else {
+__device__ __forceinline__ void set_limits(const Int4AttnParams& p, const Seq& s, const Rows& R, int row0, Query<D, NT>& Q, int lane) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + (lane & 15);
+        Q.lim[t] = r < R.n ? seen_by(p, s, r / R.G) : 0;
+    }
+    // later rows never see less
+    Q.lim_min = row0 < R.n ? uni(seen_by(p, s, row0 / R.G)) : 0x7fffffff;
+    Q.lim_max = row0 < R.n ? uni(seen_by(p, s, (min(row0 + 16 * NT, R.n) - 1) / R.G)) : 0;
+}
+// The lane's channels of q rows [row0, row0 + 16 NT) of an item, as they lie in memory.
+template <int D, int NT> struct RawQuery { uint32_t w[NT][D / 8]; };
+template <int D, int NT>
+__device__ __forceinline__ void load_query(const Int4AttnParams& p, const Rows& R, int row0, RawQuery<D, NT>& q, int lane) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + (lane & 15);
+        const bool live = r < R.n;
+        const int i = live ? r / R.G : 0;
+        const uint16_t* src = (const uint16_t*)p.q + (long long)(R.first + i) * p.q_tok + (long long)(R.head0 + (live ? r - i * R.G : 0)) * p.q_head +
+                              (lane >> 4) * (D / 4);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) q.w[t][j] = 0u;
+        if (live && p.q_wide) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 v = *(const uint4*)(src + 8 * j);
+                q.w[t][4 * j] = v.x; q.w[t][4 * j + 1] = v.y; q.w[t][4 * j + 2] = v.z; q.w[t][4 * j + 3] = v.w;
             }
-        }
+        } else if (live) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[2 * e] = bf ? bf16_lo(w[e]) : lo16(w[e]);
-            x[2 * e + 1] = bf ? bf16_hi(w[e]) : hi16(w[e]);
+            for (int j = 0; j < D / 8; ++j) q.w[t][j] = (uint32_t)src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
         }
-    };
+    }
+}
+// -> operand B.  The rows of a wave are brought to a common power of two with the largest element in [2^10, 2^11): float16
+// then holds every element down to 2^-25 of it exactly (bfloat16 rows outside float16's range included), and the even
+// slots, 16 times larger, stay below 2^15.
+template <int D, int NT>
+__device__ __forceinline__ void make_query(const Int4AttnParams& p, const RawQuery<D, NT>& q, Query<D, NT>& Q) {
+    const bool bf = p.q_dtype == kBF16;
+    auto lo = [&](uint32_t w) { return bf ? bf16_lo(w) : lo16(w); };
+    auto hi = [&](uint32_t w) { return bf ? bf16_hi(w) : hi16(w); };
     float top = 0.f;
-    Q.lim_min = 0x7fffffff;
-    Q.lim_max = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            float x[8];
-            piece(t, j, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sum += x[e];
-                top = fmaxf(top, fabsf(x[e]));
-            }
+        for (int j = 0; j < D / 8; ++j) {
+            const float a = lo(q.w[t][j]), b = hi(q.w[t][j]);
+            sum += a + b;
+            top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
         }
         Q.sum[t] = rows_sum(sum) * (p.scale * kLog2e);
-        const int r = row0 + 16 * t + n;
-        const bool live = r < R.n;
-        Q.lim[t] = live ? seen_by(p, s, r / R.G) : 0;
-        if (live) {
-            Q.lim_min = min(Q.lim_min, Q.lim[t]);
-            Q.lim_max = max(Q.lim_max, Q.lim[t]);
-        }
     }
-    for (int d = 1; d < 64; d <<= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-        Q.lim_min = min(Q.lim_min, __shfl_xor(Q.lim_min, d));
-        Q.lim_max = max(Q.lim_max, __shfl_xor(Q.lim_max, d));
-    }
-    Q.lim_min = uni(Q.lim_min);
-    Q.lim_max = uni(Q.lim_max);
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     // exponent of the largest element (an infinite query is not scaled: its row comes out NaN)
     const int eb = (int)((__float_as_uint(top) >> 23) & 255u);
     const int up = uni(max(-118, min(118, (top > 0.f && eb < 255) ? 127 + 10 - eb : 0)));
     const float f = __uint_as_float((uint32_t)(127 + up) << 23);
     // codes arrive as c * 2^-24 (even channels) and 16 c * 2^-24 (odd); even slots of q carry 16 f, odd ones f
     Q.ks = p.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;   // 2^24 / 16
-    // (the rows are read again, from the cache, rather than kept: they would take the registers of the sums to come)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
+        for (int j = 0; j < D / 32; ++j) {
             float x[8];
-            piece(t, j, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= (e & 1) ? f : 16.f * f;
+            for (int e = 0; e < 4; ++e) {
+                x[2 * e] = lo(q.w[t][4 * j + e]) * (16.f * f);
+                x[2 * e + 1] = hi(q.w[t][4 * j + e]) * f;
+            }
             Q.q[t][j] = u32x4{pack_f16(x[0], x[4]), pack_f16(x[1], x[5]), pack_f16(x[2], x[6]), pack_f16(x[3], x[7])};
         }
 }
 
-// The data of one step: the codes of both halves, and one parameter pair per lane (lanes 0 .. 31 the K pairs of the 32
-// tokens, lanes 32 .. 63 the V pairs), which go through LDS to the lanes that need them: one load and one register for
-// what as operands takes sixteen.
-template <int D>
-struct Tile {
-    Words<D / 32> k[2], v[2];
-    uint32_t par;
+// ---- the data of a step ---------------------------------------------------------------------------------------------
+// A step's data goes from memory straight into LDS (no registers while it is under way, so several steps can be): the four
+// half tiles K0, K1, V0, V1 of 8 D bytes each as 16-byte pieces, then the parameters, K of the 32 tokens and V of them.
+// The pieces of a half lie in the order in which the lanes read them back.
+template <int D> struct Slot {
+    static constexpr int half = 8 * D, params = 32 * D, bytes = 32 * D + 256, loads = D / 32 + 1;
 };
-// par: the lane's place in the parameters of a page's first row (K for lanes 0 .. 31, V behind)
+// Loads into LDS: lane l's bytes go to dst + l * size.  Written as assembly because the compiler, which knows such a load
+// as a write to LDS, waits for all of them before the next read of LDS it cannot tell apart; here the steps are counted
+// (wait_loads).  STREAM (nt): bytes that nobody reads again soon.  (A write of m0 needs one wait state before its use.)
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+template <bool STREAM>
+__device__ __forceinline__ void pieces_to_lds(const uint8_t* base, unsigned off, void* dst) {   // base uniform
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_offset(dst)), "v"(off), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_offset(dst)), "v"(off), "s"(base) : "memory");
+}
+template <bool STREAM>
+__device__ __forceinline__ void pieces_to_lds(const uint8_t* src, void* dst) {
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_offset(dst)), "v"(src) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_offset(dst)), "v"(src) : "memory");
+}
+__device__ __forceinline__ void word_to_lds(const uint32_t* src, void* dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_offset(dst)), "v"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// par: the lane's place in the parameters of the cache's first row (K for lanes 0 .. 31, V behind)
 template <int D, bool STREAM>
-__device__ __forceinline__ void load_tile(const Int4AttnParams& p, const uint32_t* par, const Ptrs& a, Tile<D>& t, int lane) {
-    t.par = par[p.paired ? a.row[0] : ((lane & 16) ? a.row[1] - 16 : a.row[0])];
+__device__ __forceinline__ void fetch(const Int4AttnParams& p, const uint32_t* par, const Ptrs& a, uint8_t* slot, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+    word_to_lds(par + (p.paired ? a.row[0] : ((lane & 16) ? a.row[1] - 16 : a.row[0])), slot + Slot<D>::params);
+    if constexpr (D >= 128) {
+        // a lane's own bytes: D / 128 pieces of each half
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        t.k[i] = load_words<D / 32, STREAM>(p.kcache + a.row[i] * (D / 2) + (unsigned)((lane & 15) * (D / 2) + (lane >> 4) * (D / 8)));
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        t.v[i] = load_words<D / 32, STREAM>(p.vcache + a.row[i] * (D / 2) + (unsigned)((lane >> 4) * (2 * D) + (lane & 15) * (D / 8)));
+            for (int c = 0; c < D / 128; ++c) {
+                const unsigned ko = n * (D / 2) + kg * (D / 8) + c * 16, vo = kg * (2 * D) + n * (D / 8) + c * 16;
+                pieces_to_lds<STREAM>(p.kcache + a.row[i] * (D / 2), ko, slot + (i * (D / 128) + c) * 1024);
+                pieces_to_lds<STREAM>(p.vcache + a.row[i] * (D / 2), vo, slot + 2 * Slot<D>::half + (i * (D / 128) + c) * 1024);
+            }
+    } else if constexpr (D == 64) {
+        // 32 pieces a half: K by (half of a token's row, token), V as it lies in memory
+        const long long row = (lane & 32) ? a.row[1] : a.row[0];
+        pieces_to_lds<STREAM>(p.kcache + row * (D / 2) + (n * 32 + (kg & 1) * 16), slot);
+        pieces_to_lds<STREAM>(p.vcache + row * (D / 2) + (lane & 31) * 16, slot + 2 * Slot<D>::half);
+    } else {
+        // 16 pieces a half, all four halves in one load
+        const long long row = (lane & 16) ? a.row[1] : a.row[0];
+        pieces_to_lds<STREAM>((lane < 32 ? p.kcache : p.vcache) + row * (D / 2) + n * 16, slot);
+    }
+}
+template <int D>
+__device__ __forceinline__ Words<D / 32> k_words(const uint8_t* slot, int i, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+    const uint8_t* at = slot + i * Slot<D>::half;
+    if constexpr (D == 256) {
+        const Words<4> a = load_words<4>(at + lane * 16), b = load_words<4>(at + 1024 + lane * 16);
+        return Words<8>{{a.w[0], a.w[1], a.w[2], a.w[3], b.w[0], b.w[1], b.w[2], b.w[3]}};
+    } else if constexpr (D == 128) return load_words<4>(at + lane * 16);
+    else if constexpr (D == 64) return load_words<2>(at + ((kg >> 1) * 16 + n) * 16 + (kg & 1) * 8);
+    else return load_words<1>(at + n * 16 + kg * 4);
+}
+template <int D>
+__device__ __forceinline__ Words<D / 32> v_words(const uint8_t* slot, int i, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+    const uint8_t* at = slot + (2 + i) * Slot<D>::half;
+    if constexpr (D >= 128) return k_words<D>(slot, 2 + i, lane);
+    else return load_words<D / 32>(at + kg * (2 * D) + n * (D / 8));
 }
 struct Params { u32x4 k[2], v[2]; };     // of the lane's four tokens in each half
-__device__ __forceinline__ Params spread_params(uint32_t par, uint32_t* stage, int lane) {
-    // LDS serves a wave in order: neither the write after the reads of the step before nor these reads after the write
-    // need a wait, only the compiler has to keep the order (the first product runs while they are on their way)
-    asm volatile("" ::: "memory");
-    stage[lane] = par;
-    asm volatile("" ::: "memory");
-    const u32x4* at = (const u32x4*)(stage + (lane >> 4) * 4);
-    const Params r{{at[0], at[4]}, {at[8], at[12]}};
-    asm volatile("" ::: "memory");
-    return r;
+template <int D>
+__device__ __forceinline__ Params params_of(const uint8_t* slot, int lane) {
+    const u32x4* at = (const u32x4*)(slot + Slot<D>::params) + (lane >> 4);
+    return Params{{at[0], at[4]}, {at[8], at[12]}};
 }
 
 // A step in three parts.  MASKED: some token of the step is hidden from some row (the end of the sequence, the causal
 // border, a page that is not there); a hidden token counts as probability 0 whatever its parameters hold.
 template <int D, int NT>
-__device__ __forceinline__ void products(const Query<D, NT>& Q, const Tile<D>& T, f32x4 (&s)[2][NT]) {
+__device__ __forceinline__ void products(const Query<D, NT>& Q, const uint8_t* slot, f32x4 (&s)[2][NT], int lane) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+        const Words<D / 32> k = k_words<D>(slot, i, lane);
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-            const u32x4 c = codes_of(T.k[i].w[j]);
+            const u32x4 c = codes_of(k.w[j]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[i][t] = mfma(c, Q.q[t][j], s[i][t]);
         }
@@ -418,13 +546,14 @@ __device__ __forceinline__ void weights(State<D, NT>& S, const Params& P, const 
                       pack_f16(w[t][1][1], w[t][1][3])};
 }
 template <int D, int NT>
-__device__ __forceinline__ void accumulate(State<D, NT>& S, const Tile<D>& T, const u32x4 (&pb)[NT]) {
+__device__ __forceinline__ void accumulate(State<D, NT>& S, const uint8_t* slot, const u32x4 (&pb)[NT], int lane) {
+    const Words<D / 32> v0 = v_words<D>(slot, 0, lane), v1 = v_words<D>(slot, 1, lane);
     const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
     for (int t = 0; t < NT; ++t) S.r[t] = mfma(ones, pb[t], S.r[t]);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-        const u32x4 c0 = codes_of(T.v[0].w[j]), c1 = codes_of(T.v[1].w[j]);
+        const u32x4 c0 = codes_of(v0.w[j]), c1 = codes_of(v1.w[j]);
         const u32x4 even = {c0[0], c0[2], c1[0], c1[2]}, odd = {c0[1], c0[3], c1[1], c1[3]};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -602,42 +731,51 @@ __device__ __forceinline__ void merge_parts(const Int4AttnParams& p, const Rows&
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------
+// Steps under way per wave: as many as two workgroups per CU have LDS for.
+#ifndef KV_DEPTH
+#define KV_DEPTH 4
+#endif
+template <int D> constexpr int depth() { return D >= 256 ? 2 : KV_DEPTH; }
 template <int D, int NT, int RW, bool LIST>
 struct Lds {
-    static constexpr int merge = RW == 4 ? 0 : 2 * 16 * NT * (D + 2) * 4;   // two states
-    static constexpr int head = merge;
-    static constexpr int fixed = head + 16 + 1024;   // the flag, 256 bytes of parameters per wave
+    static constexpr int ring = depth<D>() * Slot<D>::bytes + 512;                      // of a wave: steps, table entries
+    static constexpr int merge = RW == 4 ? 0 : 2 * 16 * NT * (D + 2) * 4;               // two states, after the walk
+    static constexpr int head = 4 * ring > merge ? 4 * ring : merge;
+    static constexpr int fixed = head + 16;                                             // the flag
 };
-// Steps whose data is under way, and waves per SIMD that the registers of a variant are cut for.
-#ifndef KV_DEPTH1
-#define KV_DEPTH1 3
-#endif
-template <int D, int NT, int RW, bool LIST> constexpr int depth() { return RW == 1 && NT * D <= 128 && !LIST ? KV_DEPTH1 : 2; }
 
-
-// Steps [s0, s1) of an item for this wave: every (4 / RW)-th one from s0 + wave / RW.  The data of DEPTH
-// steps is in registers or on its way: a step's buffer is loaded again as soon as the step is done.  The loads are not
-// conditional (behind the end the last step is loaded again, from the cache), so that the waits between them stay exact.
+// Steps [s0, s1) of an item for this wave: every (4 / RW)-th one from s0 + wave / RW.  A step's slot is filled again as
+// soon as the step is done.  The loads are not conditional (behind the end the last step is loaded again, from the cache),
+// so that counting them is enough to know what has arrived.
 template <int D, int NT, int RW, bool LIST>
-__device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, const Query<D, NT>& Q, State<D, NT>& S,
-                                     int s0, int s1, const int2* list, int n_list, uint32_t* stage, int wave, int lane) {
-    constexpr int stride = 4 / RW, DEPTH = depth<D, NT, RW, LIST>();
+__device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int b, const Rows& R, int row0, State<D, NT>& S, int s0, int s1,
+                                     const int2* list, int n_list, uint8_t* ring, int wave, int lane) {
+    constexpr int stride = 4 / RW, DEPTH = depth<D>(), LOADS = Slot<D>::loads;
     const int seq_end = sq.len, kg = lane >> 4;
+    Query<D, NT> Q;
+    set_limits<D, NT>(p, sq, R, row0, Q, lane);
     int s = s0 + wave / RW;
     // no row of the wave sees anything from lim_max on (lists are not ordered by position: all of theirs is walked)
     if (!LIST) s1 = min(s1, (min(Q.lim_max, seq_end) + kInt4StepTokens - 1) / kInt4StepTokens);
-    if (s >= s1) return;
+    if (s >= s1) {
+        clear_state(S);
+        return;
+    }
+    RawQuery<D, NT> raw;
+    load_query<D, NT>(p, R, row0, raw, lane);
     const int last = s + (s1 - 1 - s) / stride * stride;
     const int32_t* table = p.map.block_table + (long long)b * p.map.max_page;
     const int bs = p.map.block_size;
     // page of 16 tokens: (units of 16) * ceil(2^32 / (bs / 16)) >> 32, exact below 2^22 units
     auto page_of = [&](unsigned u) { return (int)(p.page_magic ? __umulhi(u, p.page_magic) : u); };
-    // 64 table entries in one register, the 64 after them in another: a lookup is a lane read
-    int base = page_of(2u * (unsigned)s), cur = 0, nxt = 0;
-    auto entries = [&](int from) { return from + lane < p.map.max_page ? table[from + lane] : -1; };
+    // 64 table entries in a register, so that a lookup is a lane read; the next 64 come through LDS like the steps' data and
+    // have long arrived when they are needed (64 pages are at least 8 steps, more than are under way)
+    uint32_t* const window = (uint32_t*)(ring + DEPTH * Slot<D>::bytes);
+    auto entry = [&](int i) { return (const uint32_t*)table + min(i, p.map.max_page - 1); };
+    int base = page_of(2u * (unsigned)s) & ~63, cur = 0;
     if (!LIST) {
-        cur = entries(base);
-        nxt = entries(base + 64);
+        word_to_lds(entry(base + 64 + lane), window + ((base + 64) & 64));
+        cur = *(const volatile int*)entry(base + lane);        // (after the load above: both have arrived with it)
     }
     const int page_rows = p.Hkv * bs, first_row = R.kvh * bs;
     auto place = [&](int step, int i, Ptrs& a) {
@@ -651,9 +789,10 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
         } else {
             a.tok[i] = (int)(16u * u);
             while (page - base >= 64) {
-                cur = nxt;
                 base += 64;
-                nxt = entries(base + 64);
+                cur = (int)window[(base & 64) + lane];
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                word_to_lds(entry(base + 64 + lane), window + ((base + 64) & 64));
             }
             e = a.tok[i] < seq_end ? __builtin_amdgcn_readlane(cur, page - base) : -1;
         }
@@ -672,11 +811,11 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
     };
     const uint32_t* par = (lane < 32 ? p.k_params : p.v_params) + (lane & 31);
     const int end = min(seq_end, Q.lim_min);
-    auto compute = [&](const Tile<D>& T, const Ptrs& a) {
+    auto compute = [&](const uint8_t* slot, const Ptrs& a) {
         f32x4 x[2][NT];
         u32x4 pb[NT];
-        const Params P = spread_params(T.par, stage, lane);
-        products<D, NT>(Q, T, x);
+        const Params P = params_of<D>(slot, lane);
+        products<D, NT>(Q, slot, x, lane);
         const bool masked = !a.ok[0] || !a.ok[1] || max(a.tok[0], a.tok[1]) + 16 > end;
         float vs[2][4], top, vs_top;
         if (masked) {
@@ -689,24 +828,31 @@ __device__ __forceinline__ void walk(const Int4AttnParams& p, const Seq& sq, int
         if (masked || S.open || __any(top > kLazy || vs_top > (float)(2 << kScaleTop))) move_references<D, NT>(S, x, vs, vs_top);
         if (masked) weights<D, NT, true>(S, P, x, vs, pb);
         else weights<D, NT, false>(S, P, x, vs, pb);
-        accumulate<D, NT>(S, T, pb);
+        accumulate<D, NT>(S, slot, pb, lane);
     };
-    Tile<D> T[DEPTH];
     Ptrs a[DEPTH];
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
         locate(min(s + u * stride, last), a[u]);
-        load_tile<D, RW == 1>(p, par, a[u], T[u], lane);
+        fetch<D, RW == 1>(p, par, a[u], ring + u * Slot<D>::bytes, lane);
     }
+    make_query<D, NT>(p, raw, Q);       // while the first steps' data is on its way
+    clear_state(S);
 #pragma unroll 1
     while (true) {
 #pragma unroll
         for (int u = 0; u < DEPTH; ++u) {
-            compute(T[u], a[u]);
+            uint8_t* const slot = ring + u * Slot<D>::bytes;
+            wait_loads<(DEPTH - 1) * LOADS>();
+            compute(slot, a[u]);
             s += stride;
-            if (s >= s1) return;
+            if (s >= s1) {
+                wait_loads<0>();         // nothing may land in LDS after this
+                return;
+            }
             locate(min(s + (DEPTH - 1) * stride, last), a[u]);
-            load_tile<D, RW == 1>(p, par, a[u], T[u], lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the slot has been read
+            fetch<D, RW == 1>(p, par, a[u], slot, lane);
         }
     }
 }
@@ -720,17 +866,13 @@ __device__ __forceinline__ void run_item(const Int4AttnParams& p, const Seq& sq,
     const int my_row0 = row0 + wave % RW * 16 * NT;
     const int n_rows = min(p.rows_tile, R.n - row0);
     State<D, NT> S;
-    clear_state(S);
-    {
-        Query<D, NT> Q;
-        load_query<D, NT>(p, sq, R, my_row0, Q, lane);
-        walk<D, NT, RW, LIST>(p, sq, b, R, Q, S, s0, s1, list, n_list, (uint32_t*)(flag + 4) + 64 * wave, wave, lane);
-    }
+    if (RW < 4) __syncthreads();                          // the areas may still be read for the item before
+    walk<D, NT, RW, LIST>(p, sq, b, R, my_row0, S, s0, s1, list, n_list, (uint8_t*)lds + wave * Lds<D, NT, RW, LIST>::ring, wave, lane);
     settle<D, NT>(S);
     // the waves that hold the same rows merge pairwise
     float* const area[2] = {lds, lds + 16 * NT * (D + 2)};
     if (RW < 4) {
-        __syncthreads();                                  // the areas may still be read for the item before
+        __syncthreads();                                  // every wave has left its ring
         const int odd = RW == 1 ? wave & 1 : wave >> 1, which = RW == 1 ? wave >> 1 : wave & 1;
         if (odd) state_to_lds<D, NT>(S, area[which], lane);
         __syncthreads();
@@ -796,9 +938,8 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
         run_item<D, NT, RW, LIST>(p, sq, b, R, 0, s0, s1, p.workers == 1, base + share * state, base, base + state, state, p.workers,
                                     p.counters + item, list, n_list, lds, flag, wave, lane);
     } else {
-        const int T = p.map.T, B = p.map.B;
         if (p.zero_rest && p.map.query_start) {           // rows of no sequence
-            const int from = max(0, min(p.map.query_start[B], T)), lead = max(0, min(p.map.query_start[0], T));
+            const int T = p.map.T, from = max(0, min(p.map.query_start[p.map.B], T)), lead = max(0, min(p.map.query_start[0], T));
             for (long long r = blockIdx.x; r < lead + (long long)(T - from); r += gridDim.x) {
                 const long long t = r < lead ? r : from + (r - lead);
                 for (int e = threadIdx.x * 2; e < p.Hq * D; e += 512) put_out(p, t * p.Hq * D + e, 0.f, 0.f);
@@ -810,77 +951,17 @@ __global__ __launch_bounds__(256, 2) void int4_attention_kernel(const Int4AttnPa
         const int per = (p.workers + 7) / 8;
         const int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
         if (w >= p.workers) return;
-        // the line of steps: its length, and where this workgroup's piece begins
-        const bool lanes_b = B >= 16 || p.most_tiles <= 4;     // a lane per sequence, or the wave over the row tiles of each
-        long long total = 0, mine = 0;
-        for (int b0 = 0; b0 < B; b0 += lanes_b ? 64 : 1) {
-            if (lanes_b) {
-                mine = b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
-                total += wave_sum(mine);
-            } else {
-                total += head_steps_wave(p, seq_of(p.map, b0), lane);
-            }
-        }
-        total = uni(total) * p.Hkv;
-        const long long piece = max((long long)p.min_steps, (total + p.workers - 1) / p.workers);
-        long long g = (long long)w * piece;
-        const long long g1 = min(total, g + piece);
-        if (g >= g1) return;
-        int b = 0;
-        long long off = g, heads = 0;
-        if (lanes_b) {
-            for (int b0 = 0; b0 < B; b0 += 64) {
-                if (B > 64) mine = b0 + lane < B ? head_steps_lane(p, seq_of(p.map, b0 + lane)) : 0;
-                const long long incl = wave_scan(mine, lane) * p.Hkv;
-                const unsigned long long past = __ballot(incl > off);
-                if (past) {
-                    const int at = __ffsll(past) - 1;
-                    heads = __shfl(mine, at);
-                    off -= __shfl(incl, at) - heads * p.Hkv;
-                    b = b0 + at;
-                    break;
-                }
-                off -= __shfl(incl, 63);
-            }
-        } else {
-            for (;; ++b) {
-                heads = head_steps_wave(p, seq_of(p.map, b), lane);
-                if (off < heads * p.Hkv) break;
-                off -= heads * p.Hkv;
-            }
-        }
-        b = uni(b);
-        off = uni(off);
-        heads = uni(heads);
+        Piece pc;
+        if (!(p.wide_line ? find_piece<long long>(p, w, lane, pc) : find_piece<int>(p, w, lane, pc))) return;
+        const long long piece = uni(pc.size), g1 = uni(pc.g1);
+        long long g = uni(pc.g);
+        int b = pc.b, h = pc.h, rt = pc.rt, s0 = pc.s0;
         Seq sq = uniform_seq(p.map, b);
-        int h = uni((int)(off / heads));
-        off -= h * heads;
-        int rt = 0;
-        if (!p.causal) {
-            rt = (int)(off / steps_of(p, sq, 0));
-            off -= (long long)rt * steps_of(p, sq, 0);
-        } else {
-            const int nt = row_tiles(p, sq);
-            for (int r0 = 0; r0 < nt; r0 += 64) {
-                const long long tile = r0 + lane < nt ? steps_of(p, sq, r0 + lane) : 0;
-                const long long incl = wave_scan(tile, lane);
-                const unsigned long long past = __ballot(incl > off);
-                if (past) {
-                    const int at = __ffsll(past) - 1;
-                    off -= __shfl(incl - tile, at);
-                    rt = r0 + at;
-                    break;
-                }
-                off -= __shfl(incl, 63);
-            }
-        }
-        rt = uni(rt);
-        int s0 = uni((int)off);
         while (true) {
             const int n_steps = uni(steps_of(p, sq, rt));
             const int s1 = (int)min((long long)n_steps, s0 + (g1 - g));
             const long long item0 = g - s0;
-            const int w0 = uni((int)(item0 / piece)), w1 = uni((int)((item0 + n_steps - 1) / piece));
+            const int w0 = uni((int)quotient(item0, piece)), w1 = uni((int)quotient(item0 + n_steps - 1, piece));
             const Rows R{sq.first, h * p.G, p.G, h, sq.n * p.G};
             // slot 2 w + 1: the item begins in w's piece; slot 2 w: it began before
             run_item<D, NT, RW, LIST>(p, sq, b, R, rt * p.rows_tile, s0, s1, w0 == w1, p.parts + (2ll * w + (s0 == 0)) * state,

@@ -93,6 +93,7 @@ struct Int4AttnParams {
     int nt;                       // 16-row tiles a wave keeps
     int row_waves;                // 1, 2, 4: groups of rows among the four waves of a workgroup; the rest shares the tokens
     int rows_tile;                // rows of a work item: 16 * nt * row_waves
+    int wide_line;                // the steps of all items may exceed 31 bits
     int most_tiles;               // work items of one (sequence, kv head), at most
     int workers;                  // workgroups (all tokens) / workgroups per list (n_split)
     int min_steps;                // fewest 32-token steps worth a workgroup of their own
