@@ -163,7 +163,7 @@ def test_attention_plans(lib):
     (dict(q=None), "query"), (dict(q=t((5, 8, 64), F32)), "query"), (dict(q=t((5, 7, 64), F16)), "divisible"), (dict(H=0), "kv heads"),
     (dict(q=t((5, 160, 64), F16), out=t((5, 160, 64), F16)), "group"), (dict(out=t((5, 8, 64), BF16)), "attentionOut"),
     (dict(out=t((5, 8, 64), F16, 0x100000, (1024, 64, 1))), "attentionOut"), (dict(out=t((4, 8, 64), F16)), "attentionOut"),
-    (dict(out=t((5, 8, 64), F16, 0x100004)), "8 bytes"), (dict(out=None), "attentionOut"), (dict(lse=t((5, 7), F32)), "softmaxLse"),
+    (dict(out=t((5, 8, 64), F16, 0x100004)), "16 bytes"), (dict(out=None), "attentionOut"), (dict(lse=t((5, 7), F32)), "softmaxLse"),
     (dict(lse=t((5, 8), F16)), "softmaxLse"), (dict(scale=float("nan")), "scaleValue"), (dict(scale=float("inf")), "scaleValue"),
     (dict(start=t((6,), I32), most=0), "maxQueryLen"), (dict(start=t((6,), I32), most=1, lists=t((5, 2, 7), I32)), "block_position"),
     (dict(lists=t((5, 3, 7), I32)), "block_position"), (dict(lists=t((4, 2, 7), I32)), "block_position"), (dict(lists=t((5, 2, 5000), I32)), "4096"),
