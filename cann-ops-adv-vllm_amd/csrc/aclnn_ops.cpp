@@ -1554,27 +1554,43 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
     p.first_new = (const int32_t*)data_ptr(firstNewPage);
     p.B = B; p.Hkv = Hkv; p.D = D; p.C = C; p.Cp = round_up(C, 128); p.block_size = bs; p.max_page = max_page;
     p.max_new = (maxNewPages <= 0 || maxNewPages > max_page) ? max_page : (int)maxNewPages;
+    if (int4 && (long long)B * p.max_new > 0x7fffffffll / Hkv - 1024)
+        return bail(fail(ACLNN_ERR_PARAM_INVALID, "4-bit key cache: sequences x maxNewPages x heads (%d x %d x %d) must stay below 2^31", B, p.max_new, Hkv));
     p.kv_page_len = kv_page_len;
     p.block_ids = (int32_t*)data_ptr(blockIdsInout);
     int rows = 16;   // as many rows per centroid pass as the keys leave room for
     while (rows > 1 && spfa::assign_lds_bytes(rows, p.Cp, D) > 150 * 1024) --rows;
     p.rows_per_pass = rows;
     p.lds_bytes = spfa::assign_lds_bytes(rows, p.Cp, D);
-    if (p.lds_bytes > kMaxLds) return bail(fail(ACLNN_ERR_PARAM_INVALID, "%d clusters need %zu bytes of LDS (> %zu)", C, p.lds_bytes, kMaxLds));
+    if (!int4 && p.lds_bytes > kMaxLds) return bail(fail(ACLNN_ERR_PARAM_INVALID, "%d clusters need %zu bytes of LDS (> %zu)", C, p.lds_bytes, kMaxLds));
     e->device = current_device_or_none();
-    *workspaceSize = 0;
+    e->ws_zero_bytes = e->ws_bytes = int4 ? spfa::kAssignInt4Zeroed : 0;
+    *workspaceSize = e->ws_bytes;
     *executor = e;
     return ACLNN_SUCCESS;
 }
 
-aclnnStatus aclnnAssignBlockIds(void*, uint64_t, aclOpExecutor* executor, aclrtStream stream) {
+aclnnStatus aclnnAssignBlockIds(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream) {
     REQUIRE_PTR(executor, "executor");
     REQUIRE(executor->op == kOpAssign, "executor was not created by aclnnAssignBlockIdsGetWorkspaceSize");
     {
         const aclnnStatus ds = check_device(executor);
         if (ds != ACLNN_SUCCESS) { if (!executor->repeatable) delete executor; return ds; }
     }
-    return finish(executor, spfa::launch_assign(executor->assign, (hipStream_t)stream), "assign_block_ids launch");
+    if (executor->ws_bytes == 0) return finish(executor, spfa::launch_assign(executor->assign, (hipStream_t)stream), "assign_block_ids launch");
+    if (workspace == nullptr || workspaceSize < executor->ws_bytes || ((uintptr_t)workspace & 7) != 0) {
+        const unsigned long long need = executor->ws_bytes;
+        if (!executor->repeatable) delete executor;
+        return fail(ACLNN_ERR_PARAM_INVALID, "workspace of %llu bytes required, at a multiple of 8", need);
+    }
+    const ZeroPlace zp = place_zeroed_part(executor, workspace, (hipStream_t)stream);
+    hipError_t err = hipSuccess;
+    if (zp.zero) err = spfa::launch_zero(zp.base, zp.slot ? spfa::kScratchSlotBytes : executor->ws_zero_bytes, nullptr, 0, (hipStream_t)stream);
+    spfa::AssignParams p = executor->assign;
+    p.joined = zp.base;
+    if (err == hipSuccess) err = spfa::launch_assign_int4(p, (hipStream_t)stream);
+    launch_outcome(executor, zp, (hipStream_t)stream, err);
+    return finish(executor, err, "assign_block_ids launch");
 }
 
 // Phase 2 of SparsePagedFusionAttention for callers that cannot allocate device memory: the workspace is a fixed array

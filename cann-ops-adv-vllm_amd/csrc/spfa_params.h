@@ -78,6 +78,7 @@ struct AssignParams {
     int kv_page_len;
     int32_t* block_ids;        // [Hkv, kv_page_len] in/out
     size_t lds_bytes;
+    void* joined;              // 4-bit K: best (score, cluster) of pages whose clusters are sliced, then arrivals; zeroed before and left zeroed
 };
 
 // SparsePagedAttention (mode 0) and SparsePagedFusionAttention (mode 1).
@@ -213,6 +214,8 @@ hipError_t launch_compute_cent(const CentParams& p, hipStream_t s);
 hipError_t launch_cent_select(const CentParams& p, hipStream_t s);
 hipError_t launch_select_position(const SelectParams& p, hipStream_t s);
 hipError_t launch_assign(const AssignParams& p, hipStream_t s);
+constexpr size_t kAssignInt4Zeroed = 128 * 16 * 8 + 128 * 4;            // bytes behind AssignParams::joined
+hipError_t launch_assign_int4(const AssignParams& p, hipStream_t s);   // kv_dtype kI4 (kv_assign_int4.hip)
 // LDS of the assign kernel for rows_per_pass rows: keys, the A tile, the slot list, the centroid tiles of its 4 waves.
 size_t assign_lds_bytes(int rows_per_pass, int Cp, int D);
 // cap_out != nullptr: launch nothing, report how many workgroups of the kernel that would run can be resident.

@@ -17,7 +17,11 @@
  * key: one-tensor list holding the paged K cache, [blocks, blockSize, Hkv*D], [blocks, blockSize, Hkv, D] or
  * [blocks, Hkv, blockSize, D]; f16 / bf16 (same dtype as l1Cent) or int8.  blockTable [>=B, maxPage] i32, seqLen [B] i32,
  * firstNewPage [B] i32, l1Cent [Hkv, C, D] f16 | bf16, blockIdsInout [Hkv, kvPageLen] i32.  maxNewPages <= 0 means
- * "all pages of the block table".  Workspace size is 0.
+ * "all pages of the block table".  Workspace size is 0, but for a 4-bit key cache (below).
+ *
+ * 4-bit key cache (aclnn_append_kv_cache.h): key is uint8 [blocks, Hkv, blockSize, D / 2] with D <= 256 and blockSize a
+ * multiple of 16, antiquantScale its parameters, float16 [blocks, Hkv, blockSize, 2] (scale, zero of every token), and
+ * antiquantOffset is absent: K = scale * code + zero.  A page with a NaN parameter in a live token takes cluster 0.
  */
 #ifndef SPFA_ACLNN_ASSIGN_BLOCK_IDS_H_
 #define SPFA_ACLNN_ASSIGN_BLOCK_IDS_H_
