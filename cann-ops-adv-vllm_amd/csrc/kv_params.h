@@ -1,5 +1,5 @@
 // Launch descriptors of the KV-cache operators (append, read back, attention over a 4-bit cache), shared by the host
-// planner (aclnn_kv_ops.inc) and the kernels (kv_cache.hip, kv_attn_int4.hip).
+// planner (aclnn_kv_ops.inc) and the kernels (kv_cache.hip, kv_assign_int4.hip, kv_attn_int4.inc).
 //
 // The 4-bit cache.  A token of a kv head is D codes 0 .. 15 and a pair (scale, zero) of float16: x = scale * code + zero.
 //   K codes  uint8 [blocks, Hkv, bs, D / 2]         byte i of a token: channel 2 i (low bits), channel 2 i + 1 (high bits)
