@@ -224,3 +224,31 @@ def test_python_surface_refuses_host_tensors():
         custom_ops.empty_int4_cache(4, 2, 16, 96, device="cpu")
     c = custom_ops.empty_int4_cache(4, 2, 32, 64, device="cpu")
     assert c.key_cache.shape == (4, 2, 32, 32) and c.value_cache.shape == (4, 2, 8, 32, 4) and c.key_params.shape == (4, 2, 32, 2)
+
+
+def test_more_rows_than_a_launch_counts(lib):
+    """Rows x heads of a group beyond 2^26: refused, one less is taken."""
+    T = 1 << 20
+    wide = dict(cache4(H=1), H=1, start=t((6,), I32), most=T)
+    st, _, msg = attention(lib, q=t((T + 1, 64, 64), F16), out=t((T + 1, 64, 64), F16), **wide)
+    assert st == INVALID and "2^26" in msg
+    assert attention(lib, q=t((T, 64, 64), F16), out=t((T, 64, 64), F16), **wide)[0] == 0
+
+
+def test_assign_counts(lib):
+    """Sequences x new pages x heads beyond 2^31."""
+    L = lib
+
+    def go(B, width, most):
+        keys = L.aclCreateTensorList((c_void_p * 1)(make(L, t((9, 2, 32, 32), U8))), 1)
+        ws, ex = c_uint64(0), c_void_p(0)
+        st = L.aclnnAssignBlockIdsGetWorkspaceSize(keys, make(L, t((B, width), I32)), make(L, t((B,), I32)), make(L, t((B,), I32)),
+                                                   make(L, t((2, 100, 64), F16)), make(L, t((9, 2, 32, 2), F16)), None, 32, most,
+                                                   make(L, t((2, 9), I32)), ctypes.byref(ws), ctypes.byref(ex))
+        if ex.value:
+            L.aclDestroyAclOpExecutor(ex)
+        return st, ws.value, (L.aclGetRecentErrMsg() or b"").decode()
+    st, _, msg = go(1 << 15, 1 << 15, 0)
+    assert st == INVALID and "2^31" in msg
+    st, ws, msg = go(1 << 15, 1 << 15, 1 << 14)
+    assert st == 0 and ws > 0, msg
