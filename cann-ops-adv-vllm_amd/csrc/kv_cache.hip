@@ -12,7 +12,7 @@ namespace {
 
 #include "spfa_common.inc"
 
-constexpr int kTokMax = 64;        // most tokens a workgroup deals with
+constexpr int kTokMax = 8;        // most tokens a workgroup deals with
 constexpr int kBatch = 2;          // rows whose loads are under way at once
 
 // Where a token of the call lives.
