@@ -294,7 +294,10 @@ def assign_block_ids(key: torch.Tensor, block_table: torch.Tensor, seq_len: torc
     kv head, the mean K row of the page (rounded to l1_cent's dtype) is scored against the head's centroids like a
     query row and the page gets the best cluster's id (ties: smallest id).  A page whose block_table entry lies outside
     the KV pool (the usual -1 of an unassigned slot) is skipped.  A decode loop calls this when a page
-    fills up and advances first_new_page itself."""
+    fills up and advances first_new_page itself.
+
+    A 4-bit key cache (uint8 [blocks, Hkv, block_size, D / 2], see kv_cache) comes with its parameters (float16
+    [blocks, Hkv, block_size, 2]) as antiquant_scale; a page with a NaN in a live token's parameters takes cluster 0."""
     _abi.native.assign(key, block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset, block_ids,
                         int(block_size), int(max_new_pages))
     return block_ids
