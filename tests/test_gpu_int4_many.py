@@ -64,3 +64,15 @@ def test_two_parts_of_the_weights():
                                             dev(c["table"]), dev(c["seq"]), c["D"] ** -0.5, 1, block_size=16, block_position=lists,
                                             out_dtype=torch.float32)
     assert ((again.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("D,bs,dtype,causal", [(128, 48, "f16", True), (64, 32, "bf16", True), (32, 16, "f16", False), (256, 16, "bf16", True)])
+def test_many_rows(D, bs, dtype, causal):
+    """512 rows x 64 heads: enough tiles for the four waves of a workgroup to share the rows."""
+    check(make(D + bs, [300, 0, 212], [300, 5, 260], 64, 8, D, bs, dtype), causal)
+
+
+@pytest.mark.parametrize("n,s,Hq,Hkv,D", [([16] * 8, [900 + 37 * i for i in range(8)], 8, 1, 64), ([9, 3, 16, 12], [3000, 70, 1200, 12], 8, 1, 128)])
+def test_rows_of_two_waves(n, s, Hq, Hkv, D):
+    """65 to 128 rows of a kv head in few items: two waves share the rows, two the tokens, parts of one item each."""
+    check(make(sum(s), n, s, Hq, Hkv, D, 32, "f16"))
