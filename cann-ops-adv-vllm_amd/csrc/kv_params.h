@@ -97,6 +97,7 @@ struct Int4AttnParams {
     int most_tiles;               // work items of one (sequence, kv head), at most
     int workers;                  // workgroups (all tokens) / workgroups per list (n_split)
     int min_steps;                // fewest 32-token steps worth a workgroup of their own
+    int item_steps;               // what an item costs besides its steps, in steps
     unsigned g_magic;             // ceil(2^32 / G), 0 for a group of one
     int paired;                   // 32 tokens never cross a page (block_size a multiple of 32)
     unsigned page_magic;          // ceil(2^32 / (block_size / 16)), 0 for a block size of 16
