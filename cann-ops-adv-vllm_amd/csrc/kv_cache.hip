@@ -13,7 +13,10 @@ namespace {
 #include "spfa_common.inc"
 
 constexpr int kTokMax = 8;        // most tokens a workgroup deals with
-constexpr int kBatch = 2;          // rows whose loads are under way at once
+// rows whose loads are under way at once: 11485 tokens into a 4-bit cache and back 85 us with two, 83 with four, 78 with six,
+// 81 with eight; into a 16-bit cache 48 us with two, 55 with six; int8 rows need registers for their parameters (1813 rows of
+// 256 channels 22 us with two, 24 with six)
+template <int KIND> constexpr int batch() { return KIND == kI4 ? 6 : 2; }
 
 // Where a token of the call lives.
 struct Place {
@@ -133,22 +136,24 @@ __device__ __forceinline__ void stream8(void* base, long long off, int dtype, co
 // Rotation of the eight channels c0 .. c0 + 7 of a row: channel c < rot turns with its partner by the angle of its pair.
 // Two rounded products and a rounded sum, contraction off: the same value whichever of the two functions takes the row.
 //
-// Turn: the angles of a lane's channels, loaded once per token; the rows of all its heads turn by them.  The partner's
-// value is read from the row again (a cache hit) with the row itself, so a row costs no exchange between lanes.
+// Turn: the angles of a lane's channels, loaded once per token; the rows of all its heads turn by them.  The partners'
+// values come from the lane that holds them.
 struct Turn {
     float c[8], s[8];     // pairs side by side: four of each; low half: s is the sine's negative
     int mode;             // 0 nothing turns, 1 low half, 2 high half, 3 pairs side by side
-    int other;            // partner's channels (modes 1 and 2), or the row's own
+    int partner;          // 4 x the lane that holds the partners (modes 1 and 2), or the lane itself
+    bool halves;          // the call turns channels with those half a rotation away
 };
 __device__ __forceinline__ void load_turn(const AppendParams& p, int c0, int cs_row, Turn* t) {
     t->mode = 0;
-    t->other = c0;
+    t->partner = 4 * lane_id();
+    t->halves = p.cos_sin && !p.interleaved;
 #pragma unroll
     for (int i = 0; i < 8; ++i) { t->c[i] = 1.f; t->s[i] = 0.f; }
     if (!p.cos_sin || c0 >= p.rot) return;
     const int half = p.rot >> 1, n = p.interleaved ? 4 : 8;
     t->mode = p.interleaved ? 3 : (c0 < half ? 1 : 2);
-    if (!p.interleaved) t->other = c0 < half ? c0 + half : c0 - half;
+    if (!p.interleaved) t->partner += c0 < half ? half / 2 : -(half / 2);       // (eight channels a lane)
     const long long at = (long long)cs_row * p.rot + (p.interleaved ? c0 >> 1 : (c0 < half ? c0 : c0 - half));
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
@@ -173,8 +178,12 @@ __device__ __forceinline__ void load_turn(const AppendParams& p, int c0, int cs_
 #pragma unroll
         for (int i = 0; i < 8; ++i) t->s[i] = -t->s[i];
 }
-__device__ __forceinline__ void apply_turn(const Turn& t, uint4 other, int dtype, float* x) {
+__device__ __forceinline__ void apply_turn(const Turn& t, uint4 own, int dtype, float* x) {
 #pragma clang fp contract(off)
+    uint4 other = own;
+    if (t.halves)         // (of the call: all lanes of a row take part, those that do not turn with themselves)
+        other = make_uint4(__builtin_amdgcn_ds_bpermute(t.partner, own.x), __builtin_amdgcn_ds_bpermute(t.partner, own.y),
+                           __builtin_amdgcn_ds_bpermute(t.partner, own.z), __builtin_amdgcn_ds_bpermute(t.partner, own.w));
     if (t.mode == 0) return;
     if (t.mode == 3) {
 #pragma unroll
@@ -333,7 +342,7 @@ struct Deal {
 // (head_split workgroups).  D / 8 consecutive lanes hold a row, eight channels each.
 //
 // What bounds it: the bytes of the rows, read and written once.  A group of lanes keeps to a token and goes through the
-// token's q and K rows (16 bits and int8: V rows too), the loads of kBatch rows under way at once, the angles loaded once
+// token's q and K rows (16 bits and int8: V rows too), the loads of several rows under way at once, the angles loaded once
 // for all of them; 4-bit V rows go by quads of tokens, so that a whole quad is one 16-byte store per lane.
 // VALU work counts next to them, so types are compiled in, addresses step and the quantiser divides by its one divisor in
 // three instructions.  A prompt of 11485 tokens (32 q heads, 8 kv heads, D = 128, 4-bit cache; 248 MB): 56 us, 4.4 TB/s, with
@@ -346,7 +355,7 @@ enum { kRowQ, kRowK, kRowV };
 template <int WHAT, int KIND, int TYPE>
 __device__ __forceinline__ int token_rows(const AppendParams& p, const Place& pl, const Turn& angles, bool turn, bool store, int t, int cs, int r, int begin,
                                           int end, int step, int lanes, int sub, int lane) {
-    constexpr int AT_ONCE = TYPE >= 0 ? kBatch : 1;
+    constexpr int AT_ONCE = TYPE >= 0 ? batch<KIND>() : 1;
     const int dtype = TYPE >= 0 ? TYPE : p.dtype, c0 = sub * 8;
     const long long head = WHAT == kRowQ ? p.q_head : (WHAT == kRowK ? p.k_head : p.v_head);
     const long long start = (long long)t * (WHAT == kRowQ ? p.q_tok : (WHAT == kRowK ? p.k_tok : p.v_tok));
@@ -354,13 +363,12 @@ __device__ __forceinline__ int token_rows(const AppendParams& p, const Place& pl
     const bool any = WHAT == kRowQ || store;
     for (; r < end; r += AT_ONCE * step) {
         const int h0 = r - begin;
-        uint4 own[AT_ONCE], other[AT_ONCE];
+        uint4 own[AT_ONCE];
         if (TYPE >= 0 && turn && any) {
-            const uint16_t* row = base + h0 * head;
+            const uint16_t* row = base + h0 * head + c0;
 #pragma unroll
             for (int b = 0; b < AT_ONCE; ++b) {
-                own[b] = *(const uint4*)(row + c0);
-                if (WHAT != kRowV) other[b] = *(const uint4*)(row + angles.other);
+                own[b] = *(const uint4*)row;
                 if (r + (b + 1) * step < end) row += step * head;        // (past the end: the last row again)
             }
         }
@@ -375,7 +383,7 @@ __device__ __forceinline__ int token_rows(const AppendParams& p, const Place& pl
                 if (turn) {
                     if (TYPE >= 0) {
                         floats8(own[b], dtype, x);
-                        if (WHAT != kRowV) apply_turn(angles, other[b], dtype, x);
+                        if (WHAT != kRowV) apply_turn(angles, own[b], dtype, x);
                     } else if (WHAT == kRowV) {
                         load8(p.v, start + h * head + c0, dtype, p.wide != 0, x);
                     } else {
