@@ -1507,6 +1507,8 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
                     antiquantScale->dims[3] == 2 && is_contiguous(antiquantScale),
                 "a 4-bit key cache needs antiquantScale: its parameters, contiguous float16 [blocks, Hkv, bs, 2]");
         REQUIRE(absent(antiquantOffset), "antiquantOffset must be absent with a 4-bit key cache (its zeros are in antiquantScale)");
+        REQUIRE((((uintptr_t)data_ptr(kc) | (uintptr_t)data_ptr(antiquantScale)) & 15) == 0,
+                "the tensors of a 4-bit cache must start at a multiple of 16 bytes");
         bsh = false;
     }
     else if (kd.size() == 3 && kd[1] == bs && kd[2] == (int64_t)Hkv * D) bsh = true;

@@ -252,3 +252,20 @@ def test_assign_counts(lib):
     assert st == INVALID and "2^31" in msg
     st, ws, msg = go(1 << 15, 1 << 15, 1 << 14)
     assert st == 0 and ws > 0, msg
+
+
+def test_assign_takes_a_4_bit_cache_as_the_other_operators_do(lib):
+    """Its tensors start at multiples of 16 bytes."""
+    def go(kc=0x100000, par=0x200000):
+        keys = lib.aclCreateTensorList((c_void_p * 1)(make(lib, t((9, 2, 32, 32), U8, kc))), 1)
+        ws, ex = c_uint64(0), c_void_p()
+        st = lib.aclnnAssignBlockIdsGetWorkspaceSize(keys, make(lib, t((5, 4), I32)), make(lib, t((5,), I32)), make(lib, t((5,), I32)),
+                                                     make(lib, t((2, 100, 64), F16)), make(lib, t((9, 2, 32, 2), F16, par)), None, 32, 0,
+                                                     make(lib, t((2, 9), I32)), ctypes.byref(ws), ctypes.byref(ex))
+        if st == 0:
+            lib.aclDestroyAclOpExecutor(ex)
+        return st, (lib.aclGetRecentErrMsg() or b"").decode()
+    assert go()[0] == 0
+    for kw in (dict(kc=0x100008), dict(par=0x200004)):
+        st, msg = go(**kw)
+        assert st == INVALID and "16 bytes" in msg, msg
