@@ -190,23 +190,48 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // gather(key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start, antiquant_scale,
-//        antiquant_offset, key_out, value_out, block_size, antiquant_mode, zero_rest)
+//        antiquant_offset, key_out, value_out, block_size, antiquant_mode, tokens, heads, head_dim, bfloat16) -> (key, value)
+// key_out None: new tensors [tokens, heads, head_dim] in float16 or bfloat16, whose rows in no sequence are zeros.
 PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 14, [&]() -> PyObject* {
+    return guarded(n, 17, [&]() -> PyObject* {
         Call c("aclnnGatherKvCache");
-        static const char* const names[11] = {"key_cache", "value_cache", "key_params", "value_params", "block_table", "seq_len",
-                                              "query_start", "antiquant_scale", "antiquant_offset", "key_out", "value_out"};
-        Desc d[11];
-        for (int i = 0; i < 11; ++i) d[i] = c.desc(a[i], names[i]);
-        const int64_t bs = integer(a[11], "block_size"), mode = integer(a[12], "antiquant_mode"), rest = integer(a[13], "zero_rest");
+        static const char* const names[9] = {"key_cache", "value_cache", "key_params", "value_params", "block_table", "seq_len",
+                                             "query_start", "antiquant_scale", "antiquant_offset"};
+        const int64_t bs = integer(a[11], "block_size"), mode = integer(a[12], "antiquant_mode"), T = integer(a[13], "num_tokens"),
+                      heads = integer(a[14], "num_key_value_heads"), D = integer(a[15], "head dim"), bf16 = integer(a[16], "bfloat16");
+        const at::Tensor *cache = c.take(a[0], names[0]), *ko = c.take(a[9], "key_out"), *vo = c.take(a[10], "value_out");
+        const bool own = ko == nullptr;
+        at::Tensor k, v;
+        if (own) {
+            if (!cache) throw Failure{"key_cache must be a tensor", true};
+            if (T < 0 || heads < 0 || D < 0) raise("gather_kv_cache: a negative number of tokens, heads or channels");
+            const auto opts = cache->options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+            k = at::empty({T, heads, D}, opts);
+            v = at::empty({T, heads, D}, opts);
+        } else {
+            k = *ko;
+            v = *vo;
+        }
+        auto result = [&]() -> PyObject* {
+            PyObject *pk = own ? THPVariable_Wrap(k) : a[9], *pv = own ? THPVariable_Wrap(v) : a[10];
+            if (!own) { Py_INCREF(pk); Py_INCREF(pv); }
+            PyObject* both = PyTuple_Pack(2, pk, pv);
+            Py_DECREF(pk);
+            Py_DECREF(pv);
+            return both;
+        };
+        if (k.dim() >= 1 && k.size(0) == 0) return result();                // no rows
+        Desc d[9];
+        for (int i = 0; i < 9; ++i) d[i] = c.desc(a[i], names[i]);
+        const Desc kd = c.desc(&k), vd = c.desc(&v);
         const c10::DeviceGuard guard(c.device());
         using Plan = aclnnStatus (*)(Desc, Desc, Desc, Desc, Desc, Desc, Desc, Desc, Desc, int64_t, int64_t, int64_t, Desc, Desc, uint64_t*,
                                      aclOpExecutor**);
         uint64_t ws = 0;
         aclOpExecutor* e = nullptr;
-        const aclnnStatus s = ((Plan)g_api.gather_ws)(d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7], d[8], bs, mode, rest, d[9], d[10], &ws, &e);
+        const aclnnStatus s = ((Plan)g_api.gather_ws)(d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7], d[8], bs, mode, own ? 1 : 0, kd, vd, &ws, &e);
         c.run(s, ws, e, g_api.gather);
-        Py_RETURN_NONE;
+        return result();
     });
 }
 

@@ -76,25 +76,24 @@ def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_ta
     out_dtype: float16 or bfloat16 (default: the cache's, the antiquant parameters' or float16)."""
     if (key_out is None) != (value_out is None):
         raise _abi.AclError("gather_kv_cache: key_out and value_out come together")
-    own_out = key_out is None
-    if own_out:
-        n = int(num_tokens) if num_tokens is not None else (seq_len.shape[0] if query_start is None else None)
-        if n is None:
-            raise _abi.AclError("gather_kv_cache: num_tokens must be given with query_start")
-        heads = int(num_key_value_heads)
+    n = heads = d = 0
+    if key_out is None:
+        if num_tokens is None:
+            if query_start is not None:
+                raise _abi.AclError("gather_kv_cache: num_tokens must be given with query_start")
+            num_tokens = seq_len.shape[0]
+        n, heads, d = int(num_tokens), int(num_key_value_heads), key_cache.shape[-1]
         if key_cache.dtype == torch.uint8:
-            d = key_cache.shape[-1] * 2
-        else:
-            d = key_cache.shape[-1] if key_cache.dim() == 4 else key_cache.shape[-1] // heads
+            d *= 2
+        elif key_cache.dim() != 4:
+            d //= heads
         if out_dtype is None:
             out_dtype = {torch.uint8: torch.float16, torch.int8: getattr(antiquant_scale, "dtype", torch.float16)}.get(
                 key_cache.dtype, key_cache.dtype)
-        key_out = torch.empty((n, heads, d), dtype=out_dtype, device=key_cache.device)
-        value_out = torch.empty_like(key_out)
-    if key_out.shape[0] > 0:
-        _abi.native.gather(key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start, antiquant_scale,
-                           antiquant_offset, key_out, value_out, block_size, antiquant_mode, own_out)
-    return key_out, value_out
+        if out_dtype not in (torch.float16, torch.bfloat16):
+            raise _abi.AclError("gather_kv_cache: out_dtype must be float16 or bfloat16")
+    return _abi.native.gather(key_cache, value_cache, key_params, value_params, block_table, seq_len, query_start, antiquant_scale,
+                              antiquant_offset, key_out, value_out, block_size, antiquant_mode, n, heads, d, out_dtype == torch.bfloat16)
 
 
 def paged_attention_int4(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, key_params: torch.Tensor,
