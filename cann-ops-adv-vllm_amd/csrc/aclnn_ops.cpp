@@ -1506,6 +1506,7 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
                     antiquantScale->dims[0] == kd[0] && antiquantScale->dims[1] == Hkv && antiquantScale->dims[2] == bs &&
                     antiquantScale->dims[3] == 2 && is_contiguous(antiquantScale),
                 "a 4-bit key cache needs antiquantScale: its parameters, contiguous float16 [blocks, Hkv, bs, 2]");
+        REQUIRE((long long)C * D < (1ll << 31), "%d clusters of %d channels: a head's centroids must stay below 4 GiB with a 4-bit key cache", C, D);
         REQUIRE(absent(antiquantOffset), "antiquantOffset must be absent with a 4-bit key cache (its zeros are in antiquantScale)");
         REQUIRE((((uintptr_t)data_ptr(kc) | (uintptr_t)data_ptr(antiquantScale)) & 15) == 0,
                 "the tensors of a 4-bit cache must start at a multiple of 16 bytes");

@@ -6,14 +6,14 @@
 // the order of the channels), and keep the best cluster of every page as they go.
 //
 // What bounds it: the pages come from HBM once, and that is the floor; but each workgroup also reads its centroids from
-// L2, and a CU takes no more than about 17 bytes a clock from there (512 KB of centroids: 13 us, whether 128 or 256
-// workgroups do it).  So as many pages as possible share a pass over the centroids, and where the pages are few (a decode
-// step's) the centroids are sliced over workgroups that each form the means again from L2; their results join by an
-// atomic maximum of (score, cluster), which no order of arrival changes.
+// L2, half a megabyte for 2048 of them.  So as many pages as possible share a pass over the centroids, and where the pages
+// are few (a decode step's) the centroids are sliced over workgroups that each form the means again from L2; their results
+// join by an atomic maximum of (score, cluster), which no order of arrival changes.
 // Which pages are new is known on the device only: every workgroup counts them and derives the split from their number.
-// Measured, D = 128, pages of 128 tokens, 8 heads x 2048 clusters (a call, launch included): 64 pages 20 us, 1024
-// pages 32 us, of which reading the pages takes 11 (64 MB, 6 TB/s) and the centroids 18.  With the scores of 16 pages kept
-// in LDS and no slices, as the kernel for the other types has it, they took 41 and 103.
+// Measured, D = 128, pages of 128 tokens, 8 heads x 2048 clusters (a call, launch included): 64 pages 18 us, 1024
+// pages 23 us, of which reading the pages takes 11 (64 MB, 6 TB/s) and the centroids 8 (18 when the lanes load them as the
+// matrix instruction wants them).  With the scores of 16 pages kept in LDS and no slices, as the kernel for the other types
+// has it, they took 41 and 103.
 #include "spfa_params.h"
 
 #include <hip/hip_runtime.h>
@@ -23,6 +23,7 @@ namespace spfa {
 namespace {
 
 #include "spfa_common.inc"
+#include "kv_lds.inc"
 
 constexpr int kRows = 32, kFew = 16;                // most pages of a workgroup; pages before slices make way for more pages
 constexpr int kSpread = 256;                        // workgroups that fill the card
@@ -130,12 +131,14 @@ __device__ __forceinline__ void join_turned(float (&best)[2][4], int (&id)[2][4]
         }
 }
 
+template <int D> constexpr int tile_bytes() { return 16 * D * 2; }           // sixteen centroids
 template <int D> constexpr int waves() { return D < 256 ? 16 : 8; }      // (D = 256 needs the registers of two)
 
 template <int D, bool BF>
 __global__ __launch_bounds__(waves<D>() * 64) void assign_int4_kernel(const AssignParams p) {
     constexpr int KS = D / 32, CH = D / 16, kWaves = waves<D>();
-    __shared__ __attribute__((aligned(16))) uint16_t a_tile[kRows * D];
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // the waves' tiles of centroids, two each, then the means
+    uint16_t* const a_tile = (uint16_t*)(smem + kWaves * 2 * tile_bytes<D>());
     __shared__ Slot slots[kRows];
     __shared__ int n_slots, n_slices, last;
     __shared__ float parts[kWaves][D];
@@ -196,6 +199,27 @@ __global__ __launch_bounds__(waves<D>() * 64) void assign_int4_kernel(const Assi
     const int R = n_slots, slices = n_slices;
     if (R <= 0) return;
 
+    // ---- centroids on their way ----
+    // A tile goes from memory straight into the wave's LDS as it lies, 1024 bytes a load: lanes that follow each other in
+    // different rows, as the matrix instruction wants them, load at a quarter of that rate (16 bytes a clock).  The 16-byte
+    // pieces of a row are permuted by the row, so that sixteen rows are read back from different banks.
+    constexpr int PIECES = D / 8, ROWS = D >= 128 ? 1 : 128 / D;      // pieces of a row; rows of 256 bytes
+    auto place = [](int r, int piece) { return piece ^ (r / ROWS & (PIECES - 1) & 15); };
+    const int slice = rest % slices, tile0 = (int)((long long)tiles * slice / slices), tile1 = (int)((long long)tiles * (slice + 1) / slices);
+    const uint8_t* const cent = (const uint8_t*)p.cent + (long long)n2 * p.C * (2 * D);      // (a head's are below 4 GiB, which the host checks)
+    char* const ring = smem + wave * 2 * tile_bytes<D>();
+    auto load = [&](int tile, int slot) {
+        if (tile >= tile1) return;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int at = k * 64 + lane, r = at / PIECES, c = min(tile * 16 + r, p.C - 1);       // (past the end: the last centroid again)
+            pieces_to_lds<false>(cent, (unsigned)c * (2u * D) + (unsigned)place(r, at % PIECES) * 16u, ring + slot * tile_bytes<D>() + k * 1024);
+        }
+    };
+    int t = __builtin_amdgcn_readfirstlane(tile0 + wave);
+    load(t, 0);
+    load(t + kWaves, 1);
+
     // ---- means; few pages: a page's steps are shared by 2 to 16 waves, whose sums join in LDS ----
     int share = 1;
     while (share < kWaves && R * share * 2 <= kWaves) share *= 2;
@@ -235,25 +259,21 @@ __global__ __launch_bounds__(waves<D>() * 64) void assign_int4_kernel(const Assi
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int k = 0; k < KS; ++k) a[h][k] = *(const uint4*)(a_tile + (16 * h + col) * D + k * 32 + kq * 8);
-    const int slice = rest % slices, tile0 = (int)((long long)tiles * slice / slices), tile1 = (int)((long long)tiles * (slice + 1) / slices);
-    const uint16_t* cent = (const uint16_t*)p.cent + (long long)n2 * p.C * D + kq * 8;
-    uint4 b[2][KS];
-    auto load = [&](uint4 (&to)[KS], int t) {
-        const uint16_t* at = cent + (long long)min(min(t, tile1 - 1) * 16 + col, p.C - 1) * D;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) to[k] = *(const uint4*)(at + k * 32);
-    };
     float best[2][4];
     int id[2][4];                                    // (0: of a page whose scores are all NaN)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) { best[h][i] = -INFINITY; id[h][i] = 0; }
-    auto score = [&](const uint4 (&at)[KS], int t) {
-        const int c = min(min(t, tile1 - 1) * 16 + col, p.C - 1);
+    auto score = [&](int slot) {
+        const int c = min(t * 16 + col, p.C - 1);
+        uint4 at[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) at[k] = *(const uint4*)(ring + slot * tile_bytes<D>() + (col * PIECES + place(col, k * 4 + kq)) * 16);
+        // (Both sixteens always, also where the second is empty: with a branch there the compiler left out the waits between the
+        // first one's last matrix instruction and the comparison that reads it, two instructions later.)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (h == 1 && R <= 16) break;
             f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -268,16 +288,13 @@ __global__ __launch_bounds__(waves<D>() * 64) void assign_int4_kernel(const Assi
             }
         }
     };
-    int t = tile0 + wave;
-    load(b[0], t);
-#pragma unroll 1
-    for (; t + kWaves < tile1; t += 2 * kWaves) {
-        load(b[1], t + kWaves);
-        score(b[0], t);
-        load(b[0], t + 2 * kWaves);                      // (past the end: the last centroid again)
-        score(b[1], t + kWaves);
+    for (int slot = 0; t < tile1; t += kWaves, slot ^= 1) {
+        if (t + kWaves < tile1) wait_loads<KS>();                     // the next tile's may be under way
+        else wait_loads<0>();
+        score(slot);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile has been read
+        load(t + 2 * kWaves, slot);
     }
-    if (t < tile1) score(b[0], t);
     // the larger score wins, of equal ones the smaller cluster: over the sixteen lanes of a row by rotating it by 1, 2, 4, 8
     join_turned<1>(best, id);
     join_turned<2>(best, id);
@@ -315,9 +332,15 @@ __global__ __launch_bounds__(waves<D>() * 64) void assign_int4_kernel(const Assi
 }
 
 template <int D>
-void launch_d(const AssignParams& p, unsigned grid, hipStream_t s) {
-    if (p.qk_dtype == kBF16) hipLaunchKernelGGL((assign_int4_kernel<D, true>), dim3(grid), dim3(waves<D>() * 64), 0, s, p);
-    else hipLaunchKernelGGL((assign_int4_kernel<D, false>), dim3(grid), dim3(waves<D>() * 64), 0, s, p);
+hipError_t launch_d(const AssignParams& p, unsigned grid, hipStream_t s) {
+    static int limits[2][kMaxDevices];
+    const size_t lds = waves<D>() * 2 * tile_bytes<D>() + kRows * D * 2;
+    const bool bf = p.qk_dtype == kBF16;
+    const hipError_t e = ensure_lds_limit(bf ? (const void*)assign_int4_kernel<D, true> : (const void*)assign_int4_kernel<D, false>, limits[bf], lds);
+    if (e != hipSuccess) return e;
+    if (bf) hipLaunchKernelGGL((assign_int4_kernel<D, true>), dim3(grid), dim3(waves<D>() * 64), lds, s, p);
+    else hipLaunchKernelGGL((assign_int4_kernel<D, false>), dim3(grid), dim3(waves<D>() * 64), lds, s, p);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -332,13 +355,12 @@ hipError_t launch_assign_int4(const AssignParams& p, hipStream_t s) {
     const unsigned grid = (unsigned)(groups * p.Hkv);
     count_launch();
     switch (p.D) {
-        case 32: launch_d<32>(p, grid, s); break;
-        case 64: launch_d<64>(p, grid, s); break;
-        case 128: launch_d<128>(p, grid, s); break;
-        case 256: launch_d<256>(p, grid, s); break;
+        case 32: return launch_d<32>(p, grid, s);
+        case 64: return launch_d<64>(p, grid, s);
+        case 128: return launch_d<128>(p, grid, s);
+        case 256: return launch_d<256>(p, grid, s);
         default: return hipErrorInvalidValue;
     }
-    return hipGetLastError();
 }
 
 }  // namespace spfa
