@@ -269,3 +269,13 @@ def test_assign_takes_a_4_bit_cache_as_the_other_operators_do(lib):
     for kw in (dict(kc=0x100008), dict(par=0x200004)):
         st, msg = go(**kw)
         assert st == INVALID and "16 bytes" in msg, msg
+
+
+def test_no_rows(lib):
+    """A call without rows plans (and will launch nothing)."""
+    start = t((6,), I32)
+    assert append(lib, key=t((0, 2, 64), F16), value=t((0, 2, 64), F16), query=t((0, 8, 64), F16, 0x200000), out=t((0, 8, 64), F16, 0x300000),
+                  start=start)[0] == 0
+    assert append(lib, key=t((0, 2, 64), F16), value=t((0, 2, 64), F16), query=None, out=None, cs=None, start=start)[0] == 0
+    assert gather(lib, k=t((0, 2, 64), BF16), v=t((0, 2, 64), BF16), start=start)[0] == 0
+    assert attention(lib, q=t((0, 8, 64), F16), out=t((0, 8, 64), F16), start=start, most=1)[0] == 0
