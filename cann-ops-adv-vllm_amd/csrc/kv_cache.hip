@@ -291,12 +291,33 @@ __device__ __forceinline__ void int8_params(const CacheView& c, int which, int n
 __device__ __forceinline__ uint2 quantise8_int8(const CacheView& c, int which, int n2, int c0, int Hkv, int D, const float* x) {
     float s[8], o[8];
     int8_params(c, which, n2, c0, Hkv, D, s, o);
+    float y[8];
+    float low = fabsf(s[0]), high = low, top = fabsf(x[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        low = fminf(low, fabsf(s[i]));
+        high = fmaxf(high, fabsf(s[i]));
+        top = fmaxf(top, fabsf(x[i]));
+    }
+    if (low >= 0x1p-60f && high <= 0x1p60f && top <= 0x1p60f) {
+        // the corrected quotient of quantise8: nothing leaves the normal range here, scales have 11 bits at most (11485 tokens
+        // into an int8 cache and back 104 us, 108 with divisions)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float r = __builtin_amdgcn_rcpf(s[i]);
+            r = fmaf(fmaf(-s[i], r, 1.f), r, r);
+            const float q0 = x[i] * r;
+            y[i] = fmaf(fmaf(-q0, s[i], x[i]), r, q0) - o[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = s[i] != 0.f ? x[i] / s[i] - o[i] : 0.f;
+    }
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        float y = s[i] != 0.f ? x[i] / s[i] - o[i] : 0.f;
-        if (!(y == y)) y = 0.f;
-        const int code = (int)rintf(fminf(fmaxf(y, -128.f), 127.f));
+        const float known = y[i] == y[i] ? y[i] : 0.f;
+        const int code = (int)rintf(fminf(fmaxf(known, -128.f), 127.f));
         w[i / 4] |= (uint32_t)(code & 255) << (8 * (i % 4));
     }
     return make_uint2(w[0], w[1]);
