@@ -42,6 +42,21 @@ def test_negative_scales(n, s, Hq, Hkv, D, decode, factor, every):
     within(c)
 
 
+@pytest.mark.parametrize("top", [60000.0, float("inf")])
+@pytest.mark.parametrize("n,s,Hq,Hkv,D", [([40], [40], 4, 2, 64), ([40], [60], 4, 2, 128), ([5], [29], 8, 1, 128), ([20], [52], 2, 2, 256)])
+def test_a_large_value_scale_reaches_only_those_who_see_it(n, s, Hq, Hkv, D, top):
+    """Rows before a token with a huge scale: within the bound of the small values that they see, and the same for whatever
+    the token's parameters hold.  (Scales of 2^-14: huge ones are 2^30 times larger, more than float16 spans.)"""
+    c = make(42, n, s, Hq, Hkv, D, 16, "f16")
+    c["vp"] = (c["vp"].float() * 2.0 ** -12).half()
+    first = s[0] - n[0] + 2                              # rows 0 and 1 do not see it, row 2 on do
+    for pos in (first, s[0] - 1):
+        c["vp"][int(c["table"][0, pos // 16]), :, pos % 16, 0] = top
+    got = within(c, slice(0, 2))
+    seen = got[2:].cpu()
+    assert bool(torch.isfinite(seen).all()) == (top < 1e5)
+
+
 def test_infinite_scales_do_not_wear_out_the_reference():
     """Many tokens with an infinite scale, each in a step of its own, behind the rows that are asked for."""
     c = make(43, [200], [200], 2, 1, 64, 16, "f16")
