@@ -1510,6 +1510,8 @@ aclnnStatus aclnnAssignBlockIdsGetWorkspaceSize(const aclTensorList* key, const 
         REQUIRE(absent(antiquantOffset), "antiquantOffset must be absent with a 4-bit key cache (its zeros are in antiquantScale)");
         REQUIRE((((uintptr_t)data_ptr(kc) | (uintptr_t)data_ptr(antiquantScale)) & 15) == 0,
                 "the tensors of a 4-bit cache must start at a multiple of 16 bytes");
+        // (the centroids go straight into LDS in pieces of 16 bytes)
+        REQUIRE(((uintptr_t)data_ptr(l1Cent) & 15) == 0, "l1_cent must start at a multiple of 16 bytes with a 4-bit key cache");
         bsh = false;
     }
     else if (kd.size() == 3 && kd[1] == bs && kd[2] == (int64_t)Hkv * D) bsh = true;

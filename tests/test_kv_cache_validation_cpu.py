@@ -279,3 +279,22 @@ def test_no_rows(lib):
     assert append(lib, key=t((0, 2, 64), F16), value=t((0, 2, 64), F16), query=None, out=None, cs=None, start=start)[0] == 0
     assert gather(lib, k=t((0, 2, 64), BF16), v=t((0, 2, 64), BF16), start=start)[0] == 0
     assert attention(lib, q=t((0, 8, 64), F16), out=t((0, 8, 64), F16), start=start, most=1)[0] == 0
+
+
+@pytest.mark.parametrize("addr", [0x300002, 0x300004, 0x300008])
+def test_assign_over_a_4_bit_cache_needs_aligned_centroids(lib, addr):
+    """The centroids go to LDS in 16-byte pieces there; a key cache of 16 bits takes them anywhere, as before."""
+    def go(kc, par, cent):
+        keys = lib.aclCreateTensorList((c_void_p * 1)(make(lib, kc)), 1)
+        ws, ex = c_uint64(0), c_void_p()
+        st = lib.aclnnAssignBlockIdsGetWorkspaceSize(keys, make(lib, t((5, 4), I32)), make(lib, t((5,), I32)), make(lib, t((5,), I32)),
+                                                     make(lib, t((2, 100, 64), F16, cent)), make(lib, par), None, 32, 0,
+                                                     make(lib, t((2, 9), I32)), ctypes.byref(ws), ctypes.byref(ex))
+        if st == 0:
+            lib.aclDestroyAclOpExecutor(ex)
+        return st, (lib.aclGetRecentErrMsg() or b"").decode()
+    int4 = (t((9, 2, 32, 32), U8), t((9, 2, 32, 2), F16))
+    assert go(*int4, 0x300010)[0] == 0
+    st, msg = go(*int4, addr)
+    assert st == INVALID and "l1_cent" in msg and "16 bytes" in msg, msg
+    assert go(t((9, 2, 32, 64), F16), None, addr)[0] == 0
