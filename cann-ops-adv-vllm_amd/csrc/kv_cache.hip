@@ -248,7 +248,10 @@ __device__ __forceinline__ uint32_t quantise8(const float* x, int lanes, int lan
         lo = fminf(lo, __shfl_xor(lo, step));
         hi = fmaxf(hi, __shfl_xor(hi, step));
     }
-    const _Float16 s = (_Float16)fminf((hi - lo) * (1.f / 15.f), 65504.f);
+    // (the corrected quotient by 15, see below, equal to the division for every mantissa: the product with 1 / 15 alone misses
+    // half-way cases between two scales.  An infinite difference makes it NaN, which fminf leaves for the bound.)
+    const float span = hi - lo, s0 = span * (1.f / 15.f);
+    const _Float16 s = (_Float16)fminf(fmaf(fmaf(-s0, 15.f, span), 1.f / 15.f, s0), 65504.f);
     _Float16 z = (_Float16)fminf(fmaxf(lo, -65504.f), 65504.f);
     // 16-bit inputs meet exact halves often, so the quotient has to be the correctly rounded one; the divisor is the same
     // for the row, so this takes three instructions a channel: with r the rounded reciprocal (one Newton step from within
