@@ -397,7 +397,14 @@ __attribute__((visibility("default"))) aclnnStatus spfaSetDebugBuffer(void* dev)
 // The launch plan of an executor of the two attention ops as text (for logs and tests): which kernel form and geometry,
 // how the work is dealt.  Returns the length written (without the terminator), or -1.
 int spfaDescribeExecutor(const aclOpExecutor* e, char* buf, uint64_t n) {
-    if (!e || !buf || n == 0 || (e->op != kOpAttention && e->op != kOpFusion)) return -1;
+    if (!e || !buf || n == 0 || (e->op != kOpAttention && e->op != kOpFusion && e->op != kOpInt4Attention)) return -1;
+    if (e->op == kOpInt4Attention) {
+        const spfa::Int4AttnParams& p = e->int4;
+        const int w = snprintf(buf, n, "form=int4 row_tiles=%d row_waves=%d rows_per_item=%d workgroups=%d lists=%d wide_line=%d workspace_bytes=%llu zeroed_bytes=%llu",
+                               p.nt, p.row_waves, p.rows_tile, p.workers, p.lists ? p.list_rows : 0, p.wide_line,
+                               (unsigned long long)e->ws_bytes, (unsigned long long)e->ws_zero_bytes);
+        return w < 0 ? -1 : (w < (int)n ? w : (int)n - 1);
+    }
     const spfa::AttnParams& p = e->attn;
     const bool mfma = spfa::attention_uses_mfma(p.rows_per_pass, p.kv_dtype, p.D);
     const int w = snprintf(buf, n,

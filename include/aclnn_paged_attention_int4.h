@@ -8,8 +8,9 @@
  * 64 heads.  Rows belong to sequences as in AppendKvCache (queryStart NULL: decode, one row per sequence); the i-th of n
  * rows of sequence b stands at position seqLen[b] - n + i.  causal: it sees the tokens up to its own; otherwise all
  * seqLen[b] tokens (a cache of another sequence: an encoder's states).  Tokens behind the table and pages whose table entry lies outside the pool are not
- * there.  A row that sees no token (length 0, more rows than tokens) gets zeros.  maxQueryLen: most rows of a sequence
- * (with queryStart; an upper bound is fine, the results do not depend on it).
+ * there.  A row that sees no token (length 0, more rows than tokens) gets zeros.  maxQueryLen (with queryStart): most rows
+ * of a sequence.  It decides how rows and tokens are shared out, so the exact number is the quickest; with any other one
+ * from 1 on the results are the same up to rounding (order of the sums; weights in one float16 part or two).
  *
  * blockPosition [B, Hq | Hkv, P] i32 (or NULL): logical pages of one row per sequence, as CentSelect yields them, a row
  * ending at its first entry outside the table (0x7fffffff among them); tokens from seqLen[b] on are not seen.  P <= 4096;

@@ -298,3 +298,27 @@ def test_assign_over_a_4_bit_cache_needs_aligned_centroids(lib, addr):
     st, msg = go(*int4, addr)
     assert st == INVALID and "l1_cent" in msg and "16 bytes" in msg, msg
     assert go(t((9, 2, 32, 64), F16), None, addr)[0] == 0
+
+
+def describe(L, fn, args):
+    L.spfaDescribeExecutor.argtypes = [c_void_p, c_char_p, c_uint64]
+    ws, ex = c_uint64(0), c_void_p()
+    st = fn(*[make(L, a) if isinstance(a, (Desc, type(None))) else a for a in args], ctypes.byref(ws), ctypes.byref(ex))
+    assert st == 0, L.aclGetRecentErrMsg()
+    buf = ctypes.create_string_buffer(512)
+    n = L.spfaDescribeExecutor(ex, buf, 512)
+    L.aclDestroyAclOpExecutor(ex)
+    assert n > 0
+    return dict(part.split("=") for part in buf.value.decode().split())
+
+
+@pytest.mark.parametrize("most", [1, 3, 1 << 20])
+def test_a_bound_on_rows_does_not_shorten_the_arithmetic(lib, most):
+    """2^20 rows over tables of 2^26 tokens may be more than 2^31 steps, whatever maxQueryLen says of them."""
+    def go(T, pages):
+        c = cache4(H=1)
+        args = [t((T, 64, 64), F16), c["kc"], c["vc"], c["kp"], c["vp"], t((5, pages), I32), t((5,), I32), t((6,), I32), None, 0.125, 1, 32, most,
+                1, 1, t((T, 64, 64), F16), None]
+        return describe(lib, lib.aclnnPagedAttentionInt4GetWorkspaceSize, args)
+    assert go(1 << 20, 1 << 21)["wide_line"] == "1"
+    assert go(1 << 10, 1 << 10)["wide_line"] == "0"
