@@ -13,8 +13,7 @@
  * from 1 on the results are the same up to rounding (order of the sums; weights in one float16 part or two).
  *
  * blockPosition [B, Hq | Hkv, P] i32 (or NULL): logical pages of one row per sequence, as CentSelect yields them, a row
- * ending at its first entry outside the table (0x7fffffff among them); tokens from seqLen[b] on are not seen.  P <= 4096;
- * lists per kv head: groups of up to 64 heads (32 at D = 256).
+ * ending at its first entry outside the table (0x7fffffff among them); tokens from seqLen[b] on are not seen.  P <= 4096.
  *
  * attentionOut: query's shape, contiguous; query's dtype or float32.  softmaxLse (or NULL): float32 [T, Hq], the natural
  * logarithm of every row's sum of exponentials, -3.4e38 for a row without tokens.  zeroRest: rows in no sequence are set

@@ -322,3 +322,13 @@ def test_a_bound_on_rows_does_not_shorten_the_arithmetic(lib, most):
         return describe(lib, lib.aclnnPagedAttentionInt4GetWorkspaceSize, args)
     assert go(1 << 20, 1 << 21)["wide_line"] == "1"
     assert go(1 << 10, 1 << 10)["wide_line"] == "0"
+
+
+@pytest.mark.parametrize("D,G", [(256, 33), (256, 64), (128, 64), (32, 64)])
+def test_a_group_is_one_item_of_a_list(lib, D, G):
+    """Lists per kv head: groups of up to 64 heads at every head dim."""
+    c = cache4(H=1, D=D)
+    plan = describe(lib, lib.aclnnPagedAttentionInt4GetWorkspaceSize,
+                    [t((5, G, D), F16), c["kc"], c["vc"], c["kp"], c["vp"], t((5, 4), I32), t((5,), I32), None, t((5, 1, 7), I32), 0.1, 1, 32, 0, 1, 1,
+                     t((5, G, D), F16), None])
+    assert int(plan["rows_per_item"]) >= G and plan["lists"] == "1"
