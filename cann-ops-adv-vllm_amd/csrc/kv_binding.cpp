@@ -122,6 +122,12 @@ private:
     aclTensorList* list_ = nullptr;
 };
 
+// A call without rows launches nothing, so phase 1 does not see its operands: those that go by rows must have none either
+// (an output would come back unwritten).
+void no_rows(const at::Tensor* t, const char* name) {
+    if (t && t->numel() > 0) raise(std::string("no rows to work on, but ") + name + " holds elements");
+}
+
 int64_t integer(PyObject* o, const char* name) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
@@ -170,7 +176,12 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (given) { Py_INCREF(a[7]); return a[7]; }
             return THPVariable_Wrap(out);
         };
-        if (key->dim() == 3 && key->size(0) == 0) return result();          // no rows
+        if (key->dim() == 3 && key->size(0) == 0) {
+            no_rows(c.take(a[1], "value"), "value");
+            no_rows(query, "query");
+            no_rows(given, "query_out");
+            return result();
+        }
         const Desc kd = c.desc(key), vd = c.desc(a[1], "value"), kc = c.desc(a[2], "key_cache"), vc = c.desc(a[3], "value_cache"),
                    bt = c.desc(a[4], "block_table"), sl = c.desc(a[5], "seq_len"), qd = c.desc(query), qs = c.desc(a[8], "query_start"),
                    cs = c.desc(a[9], "cos_sin"), ps = c.desc(a[10], "positions"), sc = c.desc(a[11], "antiquant_scale"),
@@ -220,7 +231,10 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
             Py_DECREF(pv);
             return both;
         };
-        if (k.dim() >= 1 && k.size(0) == 0) return result();                // no rows
+        if (k.dim() >= 1 && k.size(0) == 0) {
+            no_rows(&v, "value_out");
+            return result();
+        }
         Desc d[9];
         for (int i = 0; i < 9; ++i) d[i] = c.desc(a[i], names[i]);
         const Desc kd = c.desc(&k), vd = c.desc(&v);
@@ -250,7 +264,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (given) { Py_INCREF(a[9]); return a[9]; }
             return THPVariable_Wrap(out);
         };
-        if (query->dim() == 3 && query->size(0) == 0) return result();
+        if (query->dim() == 3 && query->size(0) == 0) {
+            no_rows(&out, "out");
+            no_rows(c.take(a[10], "softmax_lse"), "softmax_lse");
+            return result();
+        }
         static const char* const names[9] = {"query", "key_cache", "value_cache", "key_params", "value_params", "block_table", "seq_len",
                                              "query_start", "block_position"};
         Desc d[9];
