@@ -210,4 +210,19 @@ def _bind_native():
     return mod
 
 
-native = _bind_native()
+def __getattr__(name):
+    """`native`: the binding, loaded when an operator first asks for it, so that the operators that do without it work where it
+    is not built (it needs torch's headers, the library does not)."""
+    if name == "native":
+        globals()["native"] = mod = _bind_native()
+        return mod
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def have_native() -> bool:
+    if "native" not in globals():
+        try:
+            __getattr__("native")
+        except ImportError:
+            return False
+    return True

@@ -298,8 +298,20 @@ def assign_block_ids(key: torch.Tensor, block_table: torch.Tensor, seq_len: torc
 
     A 4-bit key cache (uint8 [blocks, Hkv, block_size, D / 2], see kv_cache) comes with its parameters (float16
     [blocks, Hkv, block_size, 2]) as antiquant_scale; a page with a NaN in a live token's parameters takes cluster 0."""
-    _abi.native.assign(key, block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset, block_ids,
-                        int(block_size), int(max_new_pages))
+    if getattr(key, "dtype", None) == torch.uint8 or _abi.have_native():
+        _abi.native.assign(key, block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset, block_ids,
+                           int(block_size), int(max_new_pages))
+        return block_ids
+    # the same call through ctypes
+    _abi.require_gpu(key, block_table, seq_len, l1_cent, block_ids, first_new_page)
+    kl = _abi.to_acl_list([key])
+    descs = [_abi.to_acl(t) for t in (block_table, seq_len, first_new_page, l1_cent, antiquant_scale, antiquant_offset)]
+    ids_d = _abi.to_acl(block_ids)
+    try:
+        _abi.run(_abi.aclnnAssignBlockIdsGetWorkspaceSize, _abi.aclnnAssignBlockIds,
+                 [kl] + descs + [int(block_size), int(max_new_pages), ids_d], key.device, "aclnnAssignBlockIds")
+    finally:
+        _destroy(descs + [ids_d], [kl])
     return block_ids
 
 
