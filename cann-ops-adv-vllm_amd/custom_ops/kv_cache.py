@@ -73,11 +73,22 @@ def gather_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_ta
     """The last rows of every sequence (query_start; None: the last one) out of a paged cache of any type, in 16 bits:
     (K [T, Hkv, D], V).  num_tokens is T (needed with query_start, which lives on the GPU).  Tokens without a place in the
     cache read as zeros; rows in no sequence are zeros in new tensors and left as they are in key_out / value_out.
-    out_dtype: float16 or bfloat16 (default: the cache's, the antiquant parameters' or float16)."""
+    out_dtype: float16 or bfloat16 (default: the cache's, the antiquant parameters' or float16); where key_out is given out_dtype and
+    num_key_value_heads have to agree with it and num_tokens must not exceed its rows."""
     if (key_out is None) != (value_out is None):
         raise _abi.AclError("gather_kv_cache: key_out and value_out come together")
     n = heads = d = 0
-    if key_out is None:
+    if num_key_value_heads < 1:
+        raise _abi.AclError("gather_kv_cache: num_key_value_heads must be positive")
+    if key_out is not None:
+        # the outputs say it all: what else was said must not contradict them
+        if out_dtype not in (None, key_out.dtype):
+            raise _abi.AclError(f"gather_kv_cache: out_dtype is {out_dtype}, key_out's {key_out.dtype}")
+        if key_out.dim() == 3 and num_key_value_heads != key_out.shape[1]:
+            raise _abi.AclError(f"gather_kv_cache: num_key_value_heads is {num_key_value_heads}, key_out has {key_out.shape[1]} heads")
+        if key_out.dim() == 3 and num_tokens is not None and num_tokens > key_out.shape[0]:
+            raise _abi.AclError(f"gather_kv_cache: num_tokens is {num_tokens}, key_out has {key_out.shape[0]} rows")
+    else:
         if num_tokens is None:
             if query_start is not None:
                 raise _abi.AclError("gather_kv_cache: num_tokens must be given with query_start")

@@ -332,3 +332,18 @@ def test_a_group_is_one_item_of_a_list(lib, D, G):
                     [t((5, G, D), F16), c["kc"], c["vc"], c["kp"], c["vp"], t((5, 4), I32), t((5,), I32), None, t((5, 1, 7), I32), 0.1, 1, 32, 0, 1, 1,
                      t((5, G, D), F16), None])
     assert int(plan["rows_per_item"]) >= G and plan["lists"] == "1"
+
+
+@pytest.mark.parametrize("over,word", [(dict(out_dtype=torch.bfloat16), "out_dtype"), (dict(num_tokens=4), "num_tokens"), (dict(heads=2), "heads"),
+                                       (dict(heads=0), "heads"), (dict(heads=0, key_out=None, value_out=None), "heads")])
+def test_gather_takes_nothing_that_its_outputs_contradict(over, word):
+    import custom_ops
+    k = torch.zeros((3, 1, 64), dtype=torch.float16)
+    i = torch.zeros((3, 1), dtype=torch.int32)
+    kw = dict(key_out=k, value_out=k.clone(), heads=1)
+    kw.update(over)
+    heads = kw.pop("heads")
+    with pytest.raises(RuntimeError, match=word):
+        custom_ops.gather_kv_cache(k[None], k[None], i, i[:, 0], heads, **kw)
+    with pytest.raises(RuntimeError, match="GPU"):            # everything that agrees goes on to the next check
+        custom_ops.gather_kv_cache(k[None], k[None], i, i[:, 0], 1, key_out=k, value_out=k.clone(), out_dtype=torch.float16, num_tokens=3)
