@@ -128,6 +128,17 @@ void no_rows(const at::Tensor* t, const char* name) {
     if (t && t->numel() > 0) raise(std::string("no rows to work on, but ") + name + " holds elements");
 }
 
+// Whether two tensors' elements lie in a common range of memory.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    auto end = [](const at::Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return (const char*)t.data_ptr() + (last + 1) * t.element_size();
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    return (const char*)a.data_ptr() < end(b) && (const char*)b.data_ptr() < end(a);
+}
+
 int64_t integer(PyObject* o, const char* name) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
@@ -235,6 +246,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
             no_rows(&v, "value_out");
             return result();
         }
+        if (!own && overlap(k, v)) raise("gather_kv_cache: key_out and value_out must not overlap");
         Desc d[9];
         for (int i = 0; i < 9; ++i) d[i] = c.desc(a[i], names[i]);
         const Desc kd = c.desc(&k), vd = c.desc(&v);
@@ -269,6 +281,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             no_rows(c.take(a[10], "softmax_lse"), "softmax_lse");
             return result();
         }
+        // (query itself is fine: the rows of a work item have been read by all that share it before the last of them writes)
+        if (given && overlap(*query, out) &&
+            !(query->data_ptr() == out.data_ptr() && query->scalar_type() == out.scalar_type() && query->is_contiguous()))
+            raise("paged_attention_int4: out must be query itself or not overlap it");
         static const char* const names[9] = {"query", "key_cache", "value_cache", "key_params", "value_params", "block_table", "seq_len",
                                              "query_start", "block_position"};
         Desc d[9];

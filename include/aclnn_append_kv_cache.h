@@ -11,7 +11,8 @@
  * sequences that name the same page and row leave one of their tokens there, unspecified which.
  *
  * key, value [T, Hkv, D], query [T, Hq, D] (or NULL): f16 | bf16, channels contiguous, any token and head stride (views
- * of one projection's output).  queryOut: query's shape; it may be query itself.
+ * of one projection's output).  queryOut: query's shape; it may be query itself and
+ * overlaps nothing else.
  *
  * cosSin [positions, R] float32 or the rows' dtype, R even <= D: R / 2 cosines, then R / 2 sines (NULL: no rotation).
  * Channel pairs (i, i + R / 2), or (2 i, 2 i + 1) with interleaved, turn by the angles of the row's position —

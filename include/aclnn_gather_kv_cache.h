@@ -2,7 +2,7 @@
  * GatherKvCache: rows of a paged cache back in 16 bits — the inverse of AppendKvCache (aclnn_append_kv_cache.h): the same
  * cache types and the same naming of tokens by blockTable, seqLen and queryStart (the last n tokens of every sequence).
  *
- * keyOut, valueOut [T, Hkv, D] f16 | bf16, contiguous: x = code * scale + zero (4 bits), (code + offset) * scale (int8)
+ * keyOut, valueOut [T, Hkv, D] f16 | bf16, contiguous, not overlapping: x = code * scale + zero (4 bits), (code + offset) * scale (int8)
  * or the element itself, rounded once to the output's dtype.  A 16-bit cache has the output's dtype; int8 parameters have it too.
  * Tokens of a sequence without a place in the cache (see there) come out as zeros.  zeroRest: the same for rows in no
  * sequence; 0 leaves those as they are.  Workspace size is 0.

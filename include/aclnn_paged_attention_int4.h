@@ -15,7 +15,7 @@
  * blockPosition [B, Hq | Hkv, P] i32 (or NULL): logical pages of one row per sequence, as CentSelect yields them, a row
  * ending at its first entry outside the table (0x7fffffff among them); tokens from seqLen[b] on are not seen.  P <= 4096.
  *
- * attentionOut: query's shape, contiguous; query's dtype or float32.  softmaxLse (or NULL): float32 [T, Hq], the natural
+ * attentionOut: query's shape, contiguous; query's dtype or float32; query itself or memory of its own.  softmaxLse (or NULL): float32 [T, Hq], the natural
  * logarithm of every row's sum of exponentials, -3.4e38 for a row without tokens.  zeroRest: rows in no sequence are set
  * to zero (log-sum-exp -3.4e38); 0 leaves them as they are.
  *

@@ -347,3 +347,29 @@ def test_gather_takes_nothing_that_its_outputs_contradict(over, word):
         custom_ops.gather_kv_cache(k[None], k[None], i, i[:, 0], heads, **kw)
     with pytest.raises(RuntimeError, match="GPU"):            # everything that agrees goes on to the next check
         custom_ops.gather_kv_cache(k[None], k[None], i, i[:, 0], 1, key_out=k, value_out=k.clone(), out_dtype=torch.float16, num_tokens=3)
+
+
+def test_a_query_output_on_the_rows_it_comes_with(lib):
+    """queryOut on key's or value's rows: refused.  Rows of one projection's output lie side by side without sharing anything."""
+    base = 0x400000
+    fused = lambda heads, at: t((5, heads, 64), F16, base + 2 * 64 * at, (12 * 64, 64, 1))       # noqa: E731   q 8, k 2, v 2 heads
+    qkv = dict(query=fused(8, 0), key=fused(2, 8), value=fused(2, 10))
+    assert append(lib, **qkv, out=fused(8, 0))[0] == 0
+    assert append(lib, **qkv)[0] == 0
+    by_head = lambda heads, at: t((5, heads, 64), F16, base + 2 * 64 * 5 * at, (64, 5 * 64, 1))   # noqa: E731
+    assert append(lib, query=by_head(8, 0), key=by_head(2, 8), value=by_head(2, 10), out=by_head(8, 0))[0] == 0
+    # heads apart by more than the tokens of one, tokens of the two side by side
+    wide = lambda heads, at: t((5, heads, 64), F16, base + 2 * 64 * at, (2 * 64, 11 * 64, 1))      # noqa: E731
+    assert append(lib, query=t((5, 8, 64), F16, 0x800000), key=wide(2, 0), value=t((5, 2, 64), F16, 0x900000), out=wide(8, 1))[0] == 0
+    # heads of different widths in one token: strides differ, places in the token do not meet
+    pad = lambda heads, at, head: t((5, heads, 64), F16, base + 2 * at, (2000, head, 1))         # noqa: E731
+    assert append(lib, query=pad(8, 0, 80), key=pad(2, 640, 64), value=pad(2, 768, 64), out=pad(8, 0, 80))[0] == 0
+    assert append(lib, query=t((5, 8, 64), F16), key=pad(2, 600, 64), value=pad(2, 768, 64), out=pad(8, 0, 80))[0] == INVALID
+    one = t((5, 2, 64), F16, base + 2 * 2 * 64, (4 * 64, 64, 1))                                  # the same rows, off by half a token
+    assert append(lib, query=t((5, 2, 64), F16), key=t((5, 2, 64), F16, base, (4 * 64, 64, 1)), value=t((5, 2, 64), F16, 0x700000), out=one)[0] == 0
+    for over in (dict(out=t((5, 8, 64), F16, 0x500000), key=t((5, 2, 64), F16, 0x500000)),
+                 dict(out=t((5, 8, 64), F16, 0x500000), value=t((5, 2, 64), F16, 0x500000 - 2 * 64)),
+                 dict(qkv, query=t((5, 8, 64), F16), out=fused(8, 1)), dict(qkv, query=t((5, 8, 64), F16), out=fused(8, 3)),
+                 dict(qkv, query=t((5, 8, 64), F16), out=t((5, 8, 64), F16, base))):
+        st, _, msg = append(lib, **over)
+        assert st == INVALID and "overlap" in msg, msg
