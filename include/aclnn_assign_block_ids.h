@@ -21,7 +21,8 @@
  *
  * 4-bit key cache (aclnn_append_kv_cache.h): key is uint8 [blocks, Hkv, blockSize, D / 2] with D <= 256 and blockSize a
  * multiple of 16, antiquantScale its parameters, float16 [blocks, Hkv, blockSize, 2] (scale, zero of every token), and
- * antiquantOffset is absent: K = scale * code + zero.  All three, l1Cent too, start at multiples of 16 bytes.  A page with a NaN parameter in a live token takes cluster 0.
+ * antiquantOffset is absent: K = scale * code + zero.  key, antiquantScale and l1Cent start at multiples of 16 bytes.  A page
+ * with a NaN parameter in a live token takes cluster 0.
  */
 #ifndef SPFA_ACLNN_ASSIGN_BLOCK_IDS_H_
 #define SPFA_ACLNN_ASSIGN_BLOCK_IDS_H_

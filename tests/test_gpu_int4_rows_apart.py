@@ -3,6 +3,7 @@ of the sequence — a wave keeps up to 32 of them).  Helpers and tolerances of t
 import pytest
 import torch
 
+from oracle import kv_cache as kvo
 from test_gpu_int4_attention import call, check, make
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +48,13 @@ def test_a_query_row_that_is_not_finite_stays_alone(n, s, Hq, Hkv, D, decode, ba
     assert bool(torch.isnan(got[1]).any())
     others = torch.arange(got.shape[0], device=got.device) != 1
     assert torch.equal(got[others], base[others])
+
+
+def test_rows_near_the_end_of_bfloat16():
+    """Elements up to 2^119 times a scale of 2^-3.5: the largest score takes all, and nothing overflows on the way."""
+    c = make(33, [1, 3], [40, 90], 8, 1, 128, 32, "bf16")
+    q = rows_of(c)
+    q[::3] = torch.sign(q[::3]) * 2.0 ** 119
+    out = call(c)
+    want = kvo.attention(c["q"], kvo.values4(c["kc"], c["kp"]), kvo.values4(c["vc"], c["vp"]), c["table"], c["seq"], c["D"] ** -0.5, 1, 32, c["start"])[0]
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -6 * want.abs() + 2.0 ** -7).all()
