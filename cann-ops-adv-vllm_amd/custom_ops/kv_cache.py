@@ -119,8 +119,8 @@ def paged_attention_int4(query: torch.Tensor, key_cache: torch.Tensor, value_cac
 
     query_start None: decode, one row per sequence.  With query_start: several rows per sequence (candidate tokens, prompt
     chunks; append_kv_cache has stored their K and V), max_query_len the most rows of one sequence (default T).  It decides how
-    the work is shared out, so the exact number is the quickest — a batch of single rows planned for T rows may take twice the
-    time — while the results of any other one differ in rounding only.  causal: a row sees the tokens up to its own position;
+    the work is shared out, so the exact number is the quickest — a batch of single rows planned for T rows may take half as
+    much time again — while the results of any other one differ in rounding only.  causal: a row sees the tokens up to its own position;
     False: all seq_len[b] tokens (an encoder's states).
     block_position [B, Hq | Hkv, P] int32 (decode only): the logical pages each row attends, as cent_select returns them.
     softmax_lse: float32 [T, Hq], filled with the rows' log-sum-exp.  A row that sees no token is zero; rows in no sequence
